@@ -96,7 +96,12 @@ enum {
   MEA_ERR_LAUNCH = -8,      /* HIP reported an error at launch */
   MEA_ERR_ALIAS = -9,       /* dx overlaps another argument of mea_bwd */
   MEA_ERR_SCRATCH = -10,    /* shape needs more than MEA_STATIC_SCRATCH_BYTES */
-  MEA_ERR_DEVICE = -11      /* no current device, or the stream is another device's */
+  MEA_ERR_DEVICE = -11,     /* no current device, or the stream is another device's */
+  MEA_ERR_HEADS = -12,      /* query heads are no multiple of the key/value heads */
+  MEA_ERR_PAGE = -13,       /* page size is not 16, 32, 64, 128 or 256 */
+  MEA_ERR_DTYPE = -14,      /* element type not supported */
+  MEA_ERR_STRIDE = -15,     /* a stride is no multiple of 8 elements, or too large */
+  MEA_ERR_SCALE = -16       /* softmax scale not finite and positive */
 };
 
 /* Size of the static scratch buffer of mea_decode_static (per GPU). */
@@ -348,6 +353,156 @@ int mea_bwd_stage_grads(const mea_desc* d, const void* dy, const void* x,
                         const float* lse_save, void* daq, void* dak, void* dav,
                         void* dag, void* dO, float* delta, float* df1,
                         float* df2, void* ws, size_t ws_bytes, void* stream);
+
+/* Element types of the grouped and paged entry points. */
+enum { MEA_BF16 = 0, MEA_FP16 = 1 };
+
+/*
+ * Attention of packed sequences with grouped heads, as an operator of its own
+ * (no counterpart in the reference, whose block has as many key/value heads as
+ * query heads): query head h reads key/value head h / (Hq / Hkv), causal inside
+ * each sequence,
+ *   o_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j.
+ * Strides are in elements, multiples of 8; the N elements of a head's row are
+ * contiguous; token strides (and Hq * N) at most 2^24.
+ */
+typedef struct mea_grouped {
+  int64_t total;  /* tokens, < 2^30 */
+  int64_t nseq;   /* sequences */
+  int64_t Hq;     /* query heads, a multiple of Hkv */
+  int64_t Hkv;    /* key/value heads */
+  int64_t N;      /* head width: 32, 64, 128 or 256 */
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head; /* strides */
+  float scale;    /* > 0 */
+  int32_t dtype;  /* MEA_BF16 or MEA_FP16; the backward takes MEA_BF16 */
+} mea_grouped;
+
+/*
+ *   cu_seqlens  (nseq + 1) int32, device: nondecreasing offsets into the tokens.
+ *               Tokens before cu[0] and from cu[nseq] on belong to no sequence:
+ *               their outputs and gradients are zeros.
+ *   q           (total, Hq, N)   k, v  (total, Hkv, N)
+ *   o           (total, Hq, N), dense, out
+ *   o_rest      (total, Hq, N), dense, out: what rounding o to 16 bits left
+ *   lse         (Hq, total) fp32, out: natural-log normaliser of each row of a
+ *               sequence. o_rest and lse are what mea_grouped_bwd needs (bf16);
+ *               both NULL: not written
+ * An infinity or NaN in v reaches the rows that see its token and no others.
+ */
+int mea_grouped_fwd(const mea_grouped* d, const int32_t* cu_seqlens,
+                    const void* q, const void* k, const void* v, void* o,
+                    void* o_rest, float* lse, void* stream);
+
+/* Workspace bytes of mea_grouped_bwd; 0 when the descriptor is invalid. */
+size_t mea_grouped_workspace_bytes(const mea_grouped* d);
+
+/*
+ * Gradients of q, k and v (dense, bf16) from dout (total, Hq, N), dense, and the
+ * o, o_rest and lse that mea_grouped_fwd wrote. A key/value head's gradient is the sum
+ * over its query heads, in a fixed order. An infinity or NaN of a token may
+ * reach the gradients of any token of its sequence, and of no other.
+ */
+int mea_grouped_bwd(const mea_grouped* d, const int32_t* cu_seqlens,
+                    const void* dout, const void* q, const void* k,
+                    const void* v, const void* o, const void* o_rest,
+                    const float* lse, void* dq, void* dk, void* dv, void* ws,
+                    size_t ws_bytes, void* stream);
+
+/*
+ * A key/value cache of fixed-size pages. Sequence s holds rows
+ * 0 .. lengths[s]-1; row r lies in row r % page of page table[s][r / page] of
+ * both pools; entries past the sequence are -1. refs[p] counts the entries that
+ * hold page p (a page without any is free). The calls below change table,
+ * lengths and refs on the device, in stream order: nothing is decided on the
+ * host and nothing synchronises it. status collects what went wrong (bits, never
+ * cleared by a call). Lengths outside [0, max_pages * page] are clamped, table
+ * entries outside the pool are skipped.
+ */
+typedef struct mea_paged {
+  void *k, *v;       /* (pages, Hkv, page, N) */
+  int32_t* table;    /* (seqs, max_pages) */
+  int32_t* lengths;  /* (seqs) */
+  int32_t* refs;     /* (pages) */
+  int32_t* status;   /* (1) */
+  int64_t seqs, pages, Hkv;
+  int64_t page;      /* rows of a page: 16, 32, 64, 128 or 256 */
+  int64_t N;         /* 32, 64, 128 or 256 */
+  int64_t max_pages; /* max_pages * page < 2^30 */
+  int32_t dtype;     /* MEA_BF16 or MEA_FP16 */
+} mea_paged;
+
+/* Bits of *status. */
+enum { MEA_PAGED_NO_PAGES = 1, MEA_PAGED_NO_ROWS = 2 };
+
+/* Workspace bytes of the calls below (any of them; not of mea_tree_attn); 0
+ * when the cache is invalid. A workspace belongs to one call at a time. */
+size_t mea_paged_workspace_bytes(const mea_paged* c);
+
+/*
+ * New rows behind every sequence: n for each (cu_seqlens NULL), k and v of shape
+ * (seqs, n, Hkv, N), or cu[s+1] - cu[s] for sequence s, k and v (total, Hkv, N).
+ *   strides  six, in elements, multiples of 8: k's of sequence (unused with
+ *            cu_seqlens), token and head, then v's
+ * Sequences are served in order, each with the lowest free pages. One that
+ * finds too few (its need counts for those behind it), or would pass max_pages,
+ * stays as it is and sets MEA_PAGED_NO_PAGES or MEA_PAGED_NO_ROWS. Where the
+ * first new row falls into a page that other sequences hold too, the sequence
+ * gets a page of its own and a copy of the rows it has there.
+ */
+int mea_paged_append(const mea_paged* c, const void* k, const void* v,
+                     const int64_t* strides, const int32_t* cu_seqlens,
+                     int64_t n, int64_t total, void* ws, size_t ws_bytes,
+                     void* stream);
+
+/*
+ * Keeps the accepted tokens of a drafted tree, the last n rows of each sequence
+ * (or all of them, if it has fewer): row i of the tree becomes row path[s][i]
+ * for i < counts[s], the others go, and pages without a row are given back.
+ *   path    (seqs, most) int32, most <= n <= 256: rows of the tree, clamped to
+ *           it; any order, also twice the same
+ *   counts  (seqs) int32, clamped to [0, min(most, rows of the tree)]
+ * Pages held by other sequences too are copied first, as in mea_paged_append; a
+ * sequence without free pages for that stays as it is (MEA_PAGED_NO_PAGES).
+ */
+int mea_paged_accept(const mea_paged* c, int64_t n, const int32_t* path,
+                     int64_t most, const int32_t* counts, void* ws,
+                     size_t ws_bytes, void* stream);
+
+/* Sequence s keeps its first lengths[s] rows (at most those it has); pages
+ * without a row are given back. 0 frees the sequence. */
+int mea_paged_truncate(const mea_paged* c, const int32_t* lengths,
+                       void* stream);
+
+/* Sequence s goes on as a copy of what sequence parents[s] was before the call,
+ * sharing its pages; outside [0, seqs) it becomes empty. No row moves. */
+int mea_paged_fork(const mea_paged* c, const int32_t* parents, void* ws,
+                   size_t ws_bytes, void* stream);
+
+/* The pages in use move to the front of the pools: the k-th one behind the
+ * front (as many pages as are in use) into the k-th free one in it. */
+int mea_paged_compact(const mea_paged* c, void* ws, size_t ws_bytes,
+                      void* stream);
+
+/* Workspace bytes of mea_tree_attn (0 also where it needs none). */
+size_t mea_tree_workspace_bytes(const mea_paged* c, int64_t n, int64_t Hq);
+
+/*
+ * Attention of n new tokens per sequence over the cache, whose last n rows are
+ * the new tokens' own (mea_paged_append): token i sees every row in front of
+ * them and, of them, row j where mask[i][j] (mask NULL: j <= i). A sequence of
+ * fewer than n rows holds its last tokens' rows only. A token that sees no row
+ * gets zeros.
+ *   q          (seqs, n, Hq, N), n <= 256; q_strides: sequence, token, head
+ *   mask       (seqs, n, n) bytes, device; mask_seq: bytes between sequences (0:
+ *              one mask for all)
+ *   o          (seqs, n, Hq, N), dense, out
+ * An infinity or NaN in a v row reaches the tokens that see the row and no
+ * others.
+ */
+int mea_tree_attn(const mea_paged* c, int64_t n, int64_t Hq, float scale,
+                  const void* q, const int64_t* q_strides, const void* mask,
+                  int64_t mask_seq, void* o, void* ws, size_t ws_bytes,
+                  void* stream);
 
 /* Text for a status code returned by any entry point. */
 const char* mea_strerror(int code);

@@ -6,7 +6,9 @@ by hand-written HIP kernels in libmea.so (C ABI: include/mea.h).
 """
 from .attention import FusedAttentionFunction, FusedAttentionVarlenFunction, fused_attn, fused_attn_varlen
 from .decode import DecodeGraph, KVCache, decode_step, prefill
+from .grouped import GroupedAttentionFunction, grouped_attn_varlen
 from .module import CausalSoftmaxAttention
+from .paged import PagedKVCache, tree_attn
 from .yarn import Yarn, rotary_tables, swap_even_odd
 
 __all__ = [
@@ -19,6 +21,10 @@ __all__ = [
     "DecodeGraph",
     "prefill",
     "decode_step",
+    "GroupedAttentionFunction",
+    "grouped_attn_varlen",
+    "PagedKVCache",
+    "tree_attn",
     "Yarn",
     "rotary_tables",
     "swap_even_odd",

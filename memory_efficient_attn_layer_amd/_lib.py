@@ -40,9 +40,32 @@ class MeaDesc(ctypes.Structure):
     ]
 
 
+class MeaGrouped(ctypes.Structure):
+    """Mirror of ``struct mea_grouped``."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in ("total", "nseq", "Hq", "Hkv", "N", "q_tok", "q_head", "k_tok",
+                                                    "k_head", "v_tok", "v_head")]
+    _fields_ += [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
+class MeaPaged(ctypes.Structure):
+    """Mirror of ``struct mea_paged``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k", "v", "table", "lengths", "refs", "status")]
+    _fields_ += [(name, ctypes.c_int64) for name in ("seqs", "pages", "Hkv", "page", "N", "max_pages")]
+    _fields_ += [("dtype", ctypes.c_int32)]
+
+
+MEA_DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # MEA_BF16, MEA_FP16
+MEA_PAGED_NO_PAGES, MEA_PAGED_NO_ROWS = 1, 2
+
 _vp = ctypes.c_void_p
 _fp = ctypes.c_void_p  # float* passed as an address
 _desc = ctypes.POINTER(MeaDesc)
+_grouped = ctypes.POINTER(MeaGrouped)
+_paged = ctypes.POINTER(MeaPaged)
+_strides = ctypes.POINTER(ctypes.c_int64)
+_i64, _size = ctypes.c_int64, ctypes.c_size_t
 
 # name -> (restype, argtypes); exactly the symbols include/mea.h declares.
 EXPORTS = {
@@ -72,6 +95,20 @@ EXPORTS = {
     "mea_bwd_stage_grads": (
         ctypes.c_int,
         [_desc] + [_vp] * 7 + [_fp, _fp, _vp, _fp] + [_vp] * 5 + [_fp, _fp, _fp, _vp, ctypes.c_size_t, _vp],
+    ),
+    "mea_grouped_fwd": (ctypes.c_int, [_grouped] + [_vp] * 8),
+    "mea_grouped_workspace_bytes": (_size, [_grouped]),
+    "mea_grouped_bwd": (ctypes.c_int, [_grouped] + [_vp] * 12 + [_size, _vp]),
+    "mea_paged_workspace_bytes": (_size, [_paged]),
+    "mea_paged_append": (ctypes.c_int, [_paged, _vp, _vp, _strides, _vp, _i64, _i64, _vp, _size, _vp]),
+    "mea_paged_accept": (ctypes.c_int, [_paged, _i64, _vp, _i64, _vp, _vp, _size, _vp]),
+    "mea_paged_truncate": (ctypes.c_int, [_paged, _vp, _vp]),
+    "mea_paged_fork": (ctypes.c_int, [_paged, _vp, _vp, _size, _vp]),
+    "mea_paged_compact": (ctypes.c_int, [_paged, _vp, _size, _vp]),
+    "mea_tree_workspace_bytes": (_size, [_paged, _i64, _i64]),
+    "mea_tree_attn": (
+        ctypes.c_int,
+        [_paged, _i64, _i64, ctypes.c_float, _vp, _strides, _vp, _i64, _vp, _vp, _size, _vp],
     ),
     "mea_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "mea_version": (ctypes.c_char_p, []),

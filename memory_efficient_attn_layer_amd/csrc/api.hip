@@ -9,6 +9,7 @@
 
 #include "../../include/mea.h"
 #include "kernels.h"
+#include "launch.h"
 
 namespace {
 
@@ -165,15 +166,16 @@ T* at(void* ws, size_t off) {
 }
 
 // ---- kernel timing diagnostics -------------------------------------------
-enum KernelId {
-  K_QKVG_PROJ, K_ATTN_FWD, K_GATE_OPROJ, K_PREP, K_DZ_GATE_BWD,
-  K_ATTN_BWD_DQ, K_ATTN_BWD_DKDV, K_DW_PARTIAL, K_DW_REDUCE, K_DX,
-  K_ATTN_DECODE, K_DECODE_COMBINE, K_SKINNY_GEMM, K_TABLE_GRAD, K_TABLE_ROWS, K_COUNT
-};
+using namespace mea::kernel_ids;
+using mea::timed;
+
 const char* const kKernelNames[K_COUNT] = {
     "qkvg_proj", "attn_fwd", "gate_oproj", "prep", "dz_gate_bwd",
     "attn_bwd_dq", "attn_bwd_dkdv", "dw_partial", "dw_reduce", "dx",
-    "attn_decode", "attn_decode_combine", "skinny_gemm", "table_grad", "table_rows"};
+    "attn_decode", "attn_decode_combine", "skinny_gemm", "table_grad", "table_rows",
+    "grouped_fwd", "grouped_delta", "grouped_dq", "grouped_dkdv", "tree_attn", "tree_combine",
+    "paged_append_plan", "paged_append_rows", "paged_accept_plan", "paged_accept_rows", "paged_truncate",
+    "paged_fork_read", "paged_fork_write", "paged_compact_plan", "paged_compact_move"};
 
 struct ProfRec {
   int kernel;
@@ -196,25 +198,23 @@ hipEvent_t pool_event() {
   return e;
 }
 
-// Runs `launch` (which returns a hipError_t); when profiling is on, brackets
-// it with events on stream s.
-template <class F>
-hipError_t timed(int kernel, hipStream_t s, F launch) {
-  std::unique_lock<std::mutex> lk(g_prof_mu);
-  if (!g_prof_on || (g_prof_only >= 0 && kernel != g_prof_only)) {
-    lk.unlock();
-    return launch();
-  }
-  hipEvent_t a = pool_event(), b = pool_event();
-  if (a == nullptr || b == nullptr) return hipErrorOutOfMemory;
-  (void)hipEventRecord(a, s);
-  const hipError_t e = launch();
-  (void)hipEventRecord(b, s);
-  g_prof.push_back({kernel, a, b});
-  return e;
+}  // namespace
+
+hipError_t mea::record_begin(int kernel, hipStream_t s, TimedLaunch* t) {
+  std::lock_guard<std::mutex> lk(g_prof_mu);
+  if (!g_prof_on || (g_prof_only >= 0 && kernel != g_prof_only)) return hipSuccess;
+  t->begin = pool_event();
+  t->end = pool_event();
+  if (t->begin == nullptr || t->end == nullptr) return hipErrorOutOfMemory;
+  (void)hipEventRecord(t->begin, s);
+  return hipSuccess;
 }
 
-}  // namespace
+void mea::record_end(int kernel, hipStream_t s, const TimedLaunch& t) {
+  std::lock_guard<std::mutex> lk(g_prof_mu);
+  (void)hipEventRecord(t.end, s);
+  g_prof.push_back({kernel, t.begin, t.end});
+}
 
 extern "C" {
 
@@ -946,6 +946,11 @@ const char* mea_strerror(int code) {
     case MEA_ERR_ALIAS: return "dx overlaps another argument of the backward";
     case MEA_ERR_SCRATCH: return "the decode step needs more scratch than mea_decode_static's static buffer";
     case MEA_ERR_DEVICE: return "no current device, or the stream belongs to another device";
+    case MEA_ERR_HEADS: return "the query heads must be a multiple of the key/value heads";
+    case MEA_ERR_PAGE: return "pages must hold 16, 32, 64, 128 or 256 rows";
+    case MEA_ERR_DTYPE: return "the element type must be bf16 or fp16 (backward: bf16)";
+    case MEA_ERR_STRIDE: return "strides must be multiples of 8 elements, a row's at most 2^24";
+    case MEA_ERR_SCALE: return "the softmax scale must be finite and positive";
     default: return "unknown status";
   }
 }
