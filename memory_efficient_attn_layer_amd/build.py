@@ -40,8 +40,10 @@ HIPCC_FLAGS = [
 
 # Per-source flags. tilegemm: its kernels run one or two waves per SIMD, where
 # the compiler would keep the MFMA accumulators in AGPRs and move them between
-# register files in the main loop (232 moves; none with VGPR accumulators).
-SOURCE_FLAGS = {"tilegemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# register files in the main loop (232 moves; none with VGPR accumulators). tree:
+# one wave per SIMD, likewise.
+SOURCE_FLAGS = {"tilegemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _hipcc() -> str:

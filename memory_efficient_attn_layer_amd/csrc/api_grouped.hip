@@ -126,22 +126,24 @@ size_t paged_ws(const mea_paged* c) {
   return align_up(n * sizeof(int));
 }
 
+mea::TreeGrid tree_grid_of(const mea_paged* c, int64_t n, int64_t Hq) {
+  return mea::tree_grid((int)c->seqs, (int)c->Hkv, (int)(n * (Hq / c->Hkv)), (int)(c->max_pages * c->page), (int)c->N);
+}
+
 int check_tree(const mea_paged* c, int64_t n, int64_t Hq) {
   const int rc = check_cache(c);
   if (rc != MEA_OK) return rc;
   if (n < 1 || n > mea::kMaxTree || Hq < 1 || Hq >= 65536) return MEA_ERR_SHAPE;
   if (Hq % c->Hkv != 0) return MEA_ERR_HEADS;
-  if (c->seqs * n * Hq * (c->N / 4) / 256 + 1 >= kInt31) return MEA_ERR_SHAPE;
+  // Grid: items * Hkv by row groups; query rows in the y dimension of the second launch.
+  const mea::TreeGrid g = tree_grid_of(c, n, Hq);
+  if (n * Hq >= 65536 || g.items * g.row_groups * c->Hkv >= kInt31) return MEA_ERR_SHAPE;
   return MEA_OK;
 }
 
-int tree_split_count(const mea_paged* c, int64_t n, int64_t Hq) {
-  return mea::tree_splits((int)c->seqs, (int)c->Hkv, (int)(n * (Hq / c->Hkv)), (int)(c->max_pages * c->page), (int)c->N);
-}
-
 size_t tree_ws(const mea_paged* c, int64_t n, int64_t Hq) {
-  const int splits = tree_split_count(c, n, Hq);
-  return splits == 1 ? 0 : align_up((size_t)c->seqs * splits * n * Hq * (c->N + 4) * sizeof(float));
+  const mea::TreeGrid g = tree_grid_of(c, n, Hq);
+  return g.split ? align_up((mea::tree_head_floats((int)c->seqs) + (size_t)g.items * n * Hq * (c->N + 4)) * sizeof(float)) : 0;
 }
 
 // Checks of a call on the cache with a workspace.
@@ -321,14 +323,17 @@ int mea_tree_attn(const mea_paged* c, int64_t n, int64_t Hq, float scale, const 
   p.mask_seq = mask_seq;
   p.n = (int)n;
   p.Hq = (int)Hq;
-  p.splits = tree_split_count(c, n, Hq);
+  const mea::TreeGrid g = tree_grid_of(c, n, Hq);
+  p.want = g.want;
+  p.turn = g.turn;
+  p.row_groups = g.row_groups;
   p.sl2e = scale * 1.4426950408889634f;
   p.o = static_cast<bits16*>(o);
-  p.part = static_cast<float*>(ws);
+  p.part = g.split ? static_cast<float*>(ws) : nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool fp16 = c->dtype == MEA_FP16;
   MEA_TRY(timed(K_TREE_ATTN, s, [&] { return mea::launch_tree_attn(p, fp16, s); }));
-  if (p.splits > 1) MEA_TRY(timed(K_TREE_COMBINE, s, [&] { return mea::launch_tree_combine(p, fp16, s); }));
+  if (g.split) MEA_TRY(timed(K_TREE_COMBINE, s, [&] { return mea::launch_tree_combine(p, fp16, s); }));
   return MEA_OK;
 }
 

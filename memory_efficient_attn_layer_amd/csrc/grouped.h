@@ -81,12 +81,22 @@ struct TreeParams {
   int64_t q_seq, q_tok, q_head;
   const unsigned char* mask;  // (n, n) bytes per sequence, mask_seq apart (0: one for all); null: causal
   int64_t mask_seq;
-  int n, Hq, splits;
+  int n, Hq, want, turn, row_groups;  // the last three: of TreeGrid
   float sl2e;
   bits16* o;    // (seqs, n, Hq, N)
-  float* part;  // (seqs * Hkv, splits, rows) of N + 2 floats, rows = n * Hq / Hkv
+  // Null where no sequence can have two chunks: first item and chunks of each
+  // sequence, then (items, Hkv, rows) of N + 4 floats (the sums, m, l), rows = n * Hq / Hkv.
+  float* part;
 };
-int tree_splits(int seqs, int Hkv, int rows, int capacity, int N);
+__host__ __device__ inline size_t tree_head_floats(int seqs) { return (2 * (size_t)seqs + 3) & ~(size_t)3; }
+// How a call is cut up. split: a sequence may have several chunks, whose sums the
+// second launch joins.
+struct TreeGrid {
+  int blocks, row_groups, turn, want;
+  int64_t items;
+  bool split;
+};
+TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N);
 hipError_t launch_tree_attn(const TreeParams& p, bool fp16, hipStream_t s);
 hipError_t launch_tree_combine(const TreeParams& p, bool fp16, hipStream_t s);
 

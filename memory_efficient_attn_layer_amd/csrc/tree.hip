@@ -6,17 +6,26 @@
 //
 // Bound by reading the cache once from HBM: the rows of a key head are read for
 // all its R = n * G query rows together (row i * G + g, G query heads to a key
-// head), 32 of them to a block of v_mfma_f32_32x32x16, the query on the lane (the
-// forms of attn_fwd.hip, S^T = K Q^T, O^T += V^T P^T). A workgroup's four waves
-// are RW blocks of query rows times KG groups of keys; a tile of 32 * KG * ST keys
-// streams into LDS double-buffered and key group kg takes its own ST * 32. Few
-// query rows leave the keys to be split (flash decoding): over the key groups,
-// whose sums meet in LDS, and over `splits` workgroups of whole tiles, whose
-// fp32 sums the second launch adds in order.
+// head), 32 of them to a wave, on v_mfma_f32_32x32x16 with the query on the lane (the
+// forms of attn_fwd.hip, S^T = K Q^T, O^T += V^T P^T). Few query rows leave the keys
+// to be split (flash decoding): into chunks, one workgroup each, and over KG key
+// groups of the workgroup, which walk alternate tiles; RW waves of a group take
+// 32 query rows each of the tiles they share. Tiles stream into a ring in LDS that
+// is the group's own. A wave alone in its group (RW = 1) waits for its own loads
+// only, no barrier in the loop, and the other waves' loads stay in flight meanwhile;
+// sharing waves pass one barrier per tile. Two workgroups a CU, two waves a SIMD where
+// their registers allow it: a wave alone runs its products and exponentials one
+// after the other.
 //
-// Pages: the split's table entries are read once into LDS; each lane of a tile
-// load finds its own row's page there. Rows past the sequence and rows of pages
-// outside the pool read the pool's first row and are masked.
+// Chunks: the host knows capacities, not lengths. Every workgroup reads all
+// lengths and settles the chunk size by itself: the smallest, in whole turns of the
+// waves, that gives at most as many chunks as run at one time, so that they end
+// together. Several chunks of a sequence leave fp32 sums, which the second launch
+// adds in order.
+//
+// Pages: the chunk's table entries are read once into LDS; pages hold sixteen rows
+// or a multiple, so that every load instruction lies in one page. Rows of pages
+// outside the pool are masked.
 #include <type_traits>
 
 #include "elem.cuh"
@@ -26,26 +35,88 @@ namespace mea {
 
 namespace {
 
-// Tile geometry by head width and query blocks per workgroup.
+constexpr int kMaxChunk = 8192;             // keys
+constexpr int kTab = kMaxChunk / 16 + 2;    // its table entries at 16 rows a page
+constexpr int kSlots = 512;                 // workgroups at one time: two per CU
+
+// RW waves share a tile, KG groups of them run; rings of NS tiles that fill 64 KB.
 template <int N, int RW>
-struct Shape {
-  static constexpr int KG = N == 256 ? 2 : 4 / RW;  // key groups
-  static constexpr int ST = RW == 4 ? 2 : 1;        // 32-key steps of a group per tile
-  static constexpr int WAVES = RW * KG, BK = 32 * KG * ST;
+struct Tile {
+  static constexpr int ST = N >= 128 ? 1 : 128 / N;  // 32-key steps
+  static constexpr int KEYS = 32 * ST, ELEMS = KEYS * N;
+  static constexpr int KG = RW == 4 || N == 256 ? 1 : 2, NS = (N == 256 ? 2 : 4) / KG;
+  static constexpr int WAVES = RW * KG, LOADS = ELEMS / 8 / 64 / RW;
+  static constexpr int RING = NS * 2 * ELEMS;  // [stage][K | V]
+  static constexpr int TURN = KEYS * KG;  // keys of one turn of the workgroup
 };
-constexpr int kMaxSplitKeys = 8192;                  // keys of a split
-constexpr int kTab = kMaxSplitKeys / 16 + 2;         // its table entries at 16 rows a page
+
+// s_waitcnt vmcnt(n), and nothing that reads or writes memory moves across it.
+template <int n>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ int wave_add(int v) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// The chunk size, and the sequence and chunk that are item `item` of a head.
+struct Chunk {
+  int size, seq, chunk, count;  // seq < 0: no such item; count: the sequence's chunks (0 where it has no row)
+};
+// want: chunks of a head that run at one time; turn: granule of the size.
+__device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int turn, int item) {
+  const int lane = threadIdx.x & 63;
+  auto len = [&](int s) { return min(max(c.lengths[s], 0), c.max_pages << c.lg_page); };
+  // Up to 64 sequences stay in a register.
+  const int len0 = lane < c.seqs ? len(lane) : 0;
+  auto sum = [&](auto f) {
+    int v = lane < c.seqs ? f(len0) : 0;
+    for (int s = 64 + lane; s < c.seqs; s += 64) v += f(len(s));
+    return wave_add(v);
+  };
+  auto whole = [&](int keys) { return (keys + turn - 1) / turn * turn; };
+  Chunk r;
+  // Sums of keys in units of 16, so that they fit 32 bits.
+  const int total = sum([](int n) { return (n + 15) >> 4; });
+  r.size = min(max(whole(((total + want - 1) / want) << 4), 2 * turn), kMaxChunk);
+  while (r.size < kMaxChunk && sum([&](int n) { return max((n + r.size - 1) / r.size, 1); }) > max(want, c.seqs))
+    r.size = min(whole(r.size + r.size / 16), kMaxChunk);
+  // Item -> (sequence, chunk): every sequence has one item at least.
+  int before = 0;
+  r.seq = -1;
+  for (int s0 = 0; s0 < c.seqs; s0 += 64) {
+    const int s = s0 + lane, n = s < c.seqs ? (s0 == 0 ? len0 : len(s)) : 0;
+    const int mine = s < c.seqs ? max((n + r.size - 1) / r.size, 1) : 0;
+    int up = mine;  // inclusive
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(up, off, 64);
+      if (lane >= off) up += y;
+    }
+    const unsigned long long at = __ballot(before + up > item);
+    if (at != 0) {
+      const int l = __ffsll(at) - 1;
+      r.seq = __builtin_amdgcn_readfirstlane(s0 + l);
+      r.chunk = __builtin_amdgcn_readfirstlane(item - before - __shfl(up - mine, l, 64));
+      r.count = __builtin_amdgcn_readfirstlane((__shfl(n, l, 64) + r.size - 1) / r.size);
+      return r;
+    }
+    before += __shfl(up, 63, 64);
+  }
+  return r;
+}
 
 template <class E, int N, int RW>
-__global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kernel(TreeParams p) {
-  using S = Shape<N, RW>;
-  constexpr int KG = S::KG, ST = S::ST, WAVES = S::WAVES, BK = S::BK;
+__global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 : 2) void tree_attn_kernel(TreeParams p) {
+  using T = Tile<N, RW>;
+  constexpr int ST = T::ST, WAVES = T::WAVES, LOADS = T::LOADS, KG = T::KG, NS = T::NS;
   constexpr int CH = N / 8, KS = N / 16, DB = N / 32;
-  constexpr int TILE = BK * N;
-  constexpr int LOADS = TILE / 8 / (64 * WAVES);
-  constexpr int XCH = KG > 1 ? RW * DB * 16 * 64 * 2 : 0;  // one group's fp32 sums (16-bit elements)
-  constexpr int SMEM = 4 * TILE > XCH ? 4 * TILE : XCH;
-  __shared__ __attribute__((aligned(16))) bits16 smem[SMEM];  // [stage][K | V], then the exchange
+  static_assert(KG == 1 || KG * T::RING >= RW * DB * 16 * 64 * 2, "the exchange of one group's fp32 sums fits the rings");
+  __shared__ __attribute__((aligned(16))) bits16 smem_all[KG * T::RING];
   __shared__ int tab[kTab];
   __shared__ float xm[KG > 1 ? RW * 64 : 1], xl[KG > 1 ? RW * 64 : 1];
 
@@ -55,13 +126,15 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
   const int rw = wave % RW, kg = wave / RW;
   const int c = lane & 31, h = lane >> 5;
   const int G = p.Hq / cc.Hkv, R = p.n * G;
-  const int kv = blockIdx.x % cc.Hkv, s = blockIdx.x / cc.Hkv, split = blockIdx.y;
-  const int r0 = (blockIdx.z * RW + rw) * 32;  // this wave's query rows
+  // Key heads fastest, then the row groups that read the same rows, then chunks.
+  const int kv = blockIdx.x % cc.Hkv, grp = blockIdx.x / cc.Hkv, item = grp / p.row_groups;
+  const Chunk ck = find_chunk(cc, p.want, T::TURN, item);
+  if (ck.seq < 0) return;
+  const int s = ck.seq;
   const int len = __builtin_amdgcn_readfirstlane(min(max(cc.lengths[s], 0), cc.max_pages << cc.lg_page));
-  const int ctx = max(len - p.n, 0), lead = p.n - (len - ctx);  // lead: tokens in front of an empty sequence's rows
-  // Whole tiles per split.
-  const int per = (len + p.splits * BK - 1) / (p.splits * BK) * BK;
-  const int k_begin = split * per, k_end = min(k_begin + per, len);
+  const int ctx = max(len - p.n, 0), lead = p.n - (len - ctx);  // lead: tokens in front of a short sequence's rows
+  const int k_begin = ck.chunk * ck.size, k_end = min(k_begin + ck.size, len);
+  const int r0 = ((grp - item * p.row_groups) * RW + rw) * 32;  // first query row of the wave
 
   // Query row r = i * G + g: token i, head kv * G + g.
   const int r = min(r0 + c, R - 1), qi = r / G;
@@ -73,7 +146,7 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
   for (int db = 0; db < DB; ++db) o[db] = zero16();
 
   if (k_begin < k_end) {  // uniform over the workgroup
-    // Table entries of the split; whether all of them lie in the pool.
+    // Table entries of the chunk; whether all of them lie in the pool.
     const int first = k_begin >> cc.lg_page, pages = ((k_end - 1) >> cc.lg_page) - first + 1;
     bool ok = true;
     for (int i = tid; i < pages; i += 64 * WAVES) {
@@ -91,19 +164,39 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
       for (int ks = 0; ks < KS; ++ks) qf[ks] = ld16(qr + 16 * ks);
     }
     const size_t head_page = (size_t)cc.N << cc.lg_page;  // elements of one head's rows of a page
-    const uint32_t smem_b = lds_addr(smem);
-    auto issue_tile = [&](int j0, int stage) {
-      const uint32_t at = smem_b + (uint32_t)(stage * 2 * TILE) * 2u;
+    bits16* ring = smem_all + kg * T::RING;
+    const uint32_t ring_b = lds_addr(ring);
+    const int nt = (k_end - k_begin + T::KEYS - 1) / T::KEYS;
+    // Tile t (of the chunk) into a stage; a load instruction's rows lie in one page,
+    // so that it has a uniform base and a lane-constant offset. One of rows past the
+    // chunk, or of no page, reads the pool's first rows (the loads in flight are then
+    // always the same number).
+    uint32_t ld_off[LOADS];  // within the load's sixteen rows (bytes)
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int slot = (rw * LOADS + u) * 64 + lane, row = slot / CH;
+      ld_off[u] = (uint32_t)((row & 15) * N + ((slot % CH) ^ chunk_swz<CH>(row)) * 8) * 2u;
+    }
+    auto issue = [&](int t, int stage) {
+      const uint32_t at = ring_b + (uint32_t)(stage * 2 * T::ELEMS) * 2u;
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) {
-        const int slot = (u * WAVES + wave) * 64 + lane;
-        const int row = slot / CH, key = j0 + row;
-        const int page = key < k_end ? tab[(key >> cc.lg_page) - first] : -1;
-        const size_t off = (page < 0 ? 0 : ((size_t)page * cc.Hkv + kv) * head_page + (size_t)(key & (cc.page - 1)) * N) +
-                           ((slot % CH) ^ chunk_swz<CH>(row)) * 8;
-        g2lds16(cc.k + off, at + (uint32_t)(u * WAVES + wave) * 1024u);
-        g2lds16(cc.v + off, at + TILE * 2u + (uint32_t)(u * WAVES + wave) * 1024u);
+        const int w = rw * LOADS + u, key = k_begin + t * T::KEYS + (w * 64 / CH & ~15);  // uniform: first of sixteen rows
+        const int page = __builtin_amdgcn_readfirstlane(key < k_end ? tab[(key >> cc.lg_page) - first] : -1);
+        const size_t off = page < 0 ? 0 : ((size_t)page * cc.Hkv + kv) * head_page + (size_t)(key & (cc.page - 1)) * N;
+        g2lds16_s(cc.k + off, ld_off[u], at + (uint32_t)w * 1024u);
+        g2lds16_s(cc.v + off, ld_off[u], at + (uint32_t)T::ELEMS * 2u + (uint32_t)w * 1024u);
       }
+    };
+    // V rows of a tile that are no rows of the sequence become 0 in LDS: what lies
+    // there in the pool may be anything, and their weights are 0.
+    auto clear_tail = [&](bits16* vt, int t) {
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) {
+        const int slot = (rw * LOADS + u) * 64 + lane, key = k_begin + t * T::KEYS + slot / CH;
+        if (key >= k_end || tab[(key >> cc.lg_page) - first] < 0) *reinterpret_cast<u32x4*>(vt + slot * 8) = u32x4{0u, 0u, 0u, 0u};
+      }
+      wait_lds();
     };
 
     const int g16 = lane >> 4, i16 = lane & 15;
@@ -116,39 +209,65 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
 #pragma unroll
       for (int db = 0; db < DB; ++db) voff[x][db] = swz_off<CH>(tr_row + 8 * x, 32 * db + tr_col);
 
-    // Whether this lane's query sees row `key`.
-    const unsigned char* mrow = p.mask == nullptr ? nullptr : p.mask + s * p.mask_seq + (int64_t)qi * p.n;
-    auto sees = [&](int key) {
-      if (key >= k_end || tab[(key >> cc.lg_page) - first] < 0) return false;
-      if (key < ctx) return true;
-      const int j = key - ctx + lead;  // token of the row
-      return mrow == nullptr ? j <= qi : mrow[j] != 0;
+    // Whether the token qi sees row `key`, for the sixteen keys that this lane has
+    // of a step (bit i: key kb0 + 8 (i >> 2) + 4 h + (i & 3)). No branch in it that
+    // depends on the lane: sixteen loads in flight together.
+    const unsigned char* mask = p.mask == nullptr ? nullptr : p.mask + s * p.mask_seq;
+    auto visible = [&](int kb0, int qi) -> uint32_t {
+      uint32_t bits = 0, in = 0;
+      if (mask == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kb0 + 8 * (i >> 2) + 4 * h + (i & 3);
+          bits |= (uint32_t)(key - ctx + lead <= qi) << i;
+        }
+      } else {
+        const unsigned char* row = mask + (int64_t)qi * p.n;
+        uint32_t m[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int token = kb0 + 8 * (i >> 2) + 4 * h + (i & 3) - ctx + lead;
+          m[i] = row[min(max(token, 0), p.n - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kb0 + 8 * (i >> 2) + 4 * h + (i & 3);
+          bits |= (uint32_t)((m[i] != 0) | (key < ctx)) << i;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) in |= (uint32_t)(kb0 + 8 * (i >> 2) + 4 * h + (i & 3) < k_end) << i;
+      if (!all_in) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = min(kb0 + 8 * (i >> 2) + 4 * h + (i & 3), k_end - 1);
+          in &= ~((uint32_t)(tab[(key >> cc.lg_page) - first] < 0) << i);
+        }
+      }
+      return bits & in;
     };
 
     // One 32-key step, as in the forward of the packed prompts; MASK: some row may
     // be hidden from some query. A query that has seen no key yet has m = -inf.
-    int hidden = 0;  // masked steps whose V holds infinities or NaN, left out there
+    bool hidden = false;  // a masked step's V held infinities or NaN, left out there
     auto step = [&](const bits16* kt, const bits16* vt, int kb0, auto mask_tag) {
       constexpr bool MASK = decltype(mask_tag)::value;
-      uint32_t seen = 0xFFFFu;
-      if (MASK) {
-        seen = 0;
+      const uint32_t seen = MASK ? visible(kb0, qi) : 0;
+      auto scores = [&] {
+        f32x16 w = zero16();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) seen |= (uint32_t)sees(kb0 + 8 * (i >> 2) + 4 * h + (i & 3)) << i;
-      }
-      f32x16 w = zero16();
+        for (int ks = 0; ks < KS; ++ks) w = E::mma(*reinterpret_cast<const u32x4*>(kt + koff[ks]), qf[ks], w);
+        if (MASK) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) w = E::mma(*reinterpret_cast<const u32x4*>(kt + koff[ks]), qf[ks], w);
-      if (MASK) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if ((seen >> i & 1) == 0) w[i] = -INFINITY;
-      }
-      const f32x16 sc = w;
+          for (int i = 0; i < 16; ++i) w[i] = (seen >> i & 1) != 0 ? w[i] : -INFINITY;
+        }
+        return w;
+      };
+      f32x16 w = scores();
       float top_w;
       auto weigh = [&](float m) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = fast_exp2(__builtin_fmaf(sc[i], p.sl2e, -m));
+        for (int i = 0; i < 16; ++i) w[i] = fast_exp2(__builtin_fmaf(w[i], p.sl2e, -m));
         top_w = w[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top_w = fmaxf(top_w, w[i]);
@@ -157,9 +276,10 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
       const bool over = !(top_w <= E::kMaxWeight);
       if (__any(over)) {
         const bool up = ((int)over | __shfl_xor((int)over, 32, 64)) != 0;  // (every lane takes part in the exchange)
-        float mx = sc[0];
+        w = scores();
+        float mx = w[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, w[i]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float mn = up ? fmaxf(m_i, mx * p.sl2e) : m_i;
         const float a = mn == m_i ? 1.f : fast_exp2(m_i - mn);
@@ -168,7 +288,7 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
         for (int db = 0; db < DB; ++db) o[db] *= a;
         m_i = mn;
         // No key seen: weights exp2(-inf - 0) = 0. (NaN scores stay NaN.)
-        weigh(m_i == -INFINITY ? 0.f : m_i);
+        weigh(mn == -INFINITY ? 0.f : mn);
       }
       u32x4 pf[2];
 #pragma unroll
@@ -180,60 +300,75 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
         const bits16* vr = vt + 16 * kst * N;
         return __builtin_shufflevector(lds_read_tr4(vr + voff[0][db]), lds_read_tr4(vr + voff[1][db]), 0, 1, 2, 3);
       };
+      bool bad = false;
       if (MASK) {
         uint32_t top = 0;
 #pragma unroll
         for (int kst = 0; kst < 2; ++kst)
 #pragma unroll
           for (int db = 0; db < DB; ++db) top = max_magnitude(top, vread(kst, db));
-        if (__any(not_finite<E>(top) != 0)) {
-          hidden = 1;
-#pragma unroll
-          for (int kst = 0; kst < 2; ++kst)
-#pragma unroll
-            for (int db = 0; db < DB; ++db) o[db] = E::mma(finite_only<E>(vread(kst, db)), pf[kst], o[db]);
-          return;
-        }
+        bad = __any(not_finite<E>(top) != 0);
+        hidden = hidden || bad;
       }
 #pragma unroll
       for (int kst = 0; kst < 2; ++kst)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = E::mma(vread(kst, db), pf[kst], o[db]);
+        for (int db = 0; db < DB; ++db) {
+          u32x4 vf = vread(kst, db);
+          if (MASK && bad) vf = finite_only<E>(vf);
+          o[db] = E::mma(vf, pf[kst], o[db]);
+        }
     };
 
-    const int nt = (k_end - k_begin + BK - 1) / BK;
     // Rows that every query sees: whole steps below free_end.
     const int free_end = all_in ? min(ctx, k_end) : 0;
     const bool idle = r0 >= R;  // no query rows left for this wave
-    issue_tile(k_begin, 0);
-    wait_vmcnt0();
-    __syncthreads();
-    for (int j = 0; j < nt; ++j) {
-      const int j0 = k_begin + j * BK;
-      if (j + 1 < nt) issue_tile(j0 + BK, (j + 1) & 1);
-      const bits16* kt = smem + (j & 1) * 2 * TILE;
+#pragma unroll
+    for (int i = 0; i < NS - (RW > 1 ? 1 : 0); ++i) issue(kg + i * KG, i);
+    // RW = 1: the tile's stage is filled again once it is read. RW > 1: after the
+    // barrier that ends the wait for a tile, every wave has read the tile before it.
+    const int turns = (nt + KG - 1) / KG;
+    for (int i = 0, stage = 0; i < turns; ++i, stage = stage + 1 == NS ? 0 : stage + 1) {
+      const int t = kg + i * KG;
+      bits16* kt = ring + stage * 2 * T::ELEMS;
+      if (RW == 1)
+        wait_loads<(NS - 1) * 2 * LOADS>();
+      else
+        wait_loads<(NS - 2) * 2 * LOADS>();
+      if (!all_in || k_begin + (t + 1) * T::KEYS > k_end) clear_tail(kt + T::ELEMS, t);
+      if (RW > 1) {
+        __syncthreads();
+        issue(t + (NS - 1) * KG, stage == 0 ? NS - 1 : stage - 1);
+      }
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
-        const int row = (kg * ST + st) * 32, kb0 = j0 + row;
+        const int kb0 = k_begin + t * T::KEYS + st * 32;
         if (idle || kb0 >= k_end) continue;
         if (kb0 + 32 <= free_end)
-          step(kt + row * N, kt + TILE + row * N, kb0, std::false_type{});
+          step(kt + st * 32 * N, kt + T::ELEMS + st * 32 * N, kb0, std::false_type{});
         else
-          step(kt + row * N, kt + TILE + row * N, kb0, std::true_type{});
+          step(kt + st * 32 * N, kt + T::ELEMS + st * 32 * N, kb0, std::true_type{});
       }
-      wait_vmcnt0();
-      __syncthreads();
+      if (RW == 1) {
+        wait_lds();
+        issue(t + NS * KG, stage);
+      }
     }
+    wait_loads<0>();
     if (hidden) {  // wave-uniform: the masked steps' infinities and NaN
-      for (int j = 0; j < nt; ++j)
-        for (int st = 0; st < ST; ++st) {
-          const int kb0 = k_begin + j * BK + (kg * ST + st) * 32;
-          if (kb0 >= k_end || kb0 + 32 <= free_end) continue;
-          for (int key = kb0; key < min(kb0 + 32, k_end); ++key) {
-            const int page = tab[(key >> cc.lg_page) - first];
+      for (int t = kg; t < nt; t += KG)
+        for (int kb0 = k_begin + t * T::KEYS; kb0 < min(k_begin + (t + 1) * T::KEYS, k_end); kb0 += 32) {
+          if (kb0 + 32 <= free_end) continue;
+          const uint32_t seen = visible(kb0, qi);
+          // Bits of the lane's own half; the other half's keys come from lane ^ 32.
+          const uint32_t other = __shfl_xor(seen, 32, 64), lo = h == 0 ? seen : other, hi = h == 0 ? other : seen;
+#pragma unroll 1
+          for (int i = 0; i < 32; ++i) {
+            const int key = kb0 + i, b = (i >> 3) * 4 + (i & 3);
+            const int page = key < k_end ? tab[(key >> cc.lg_page) - first] : -1;
             if (page < 0) continue;
             const bits16* row = cc.v + ((size_t)page * cc.Hkv + kv) * head_page + (size_t)(key & (cc.page - 1)) * N + 4 * h;
-            const bool see = sees(key);
+            const bool see = ((i & 4 ? hi : lo) >> b & 1) != 0;
 #pragma unroll
             for (int db = 0; db < DB; ++db) add_not_finite<E>(o[db], row + 32 * db, see);
           }
@@ -242,41 +377,43 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
   }
 
   if constexpr (KG > 1) {
-    // The key groups' sums join group 0's, one group after the other.
-    f32x4* sx = reinterpret_cast<f32x4*>(smem) + (size_t)rw * DB * 4 * 64 + lane;
+    // The second key group's sums join the first's.
+    f32x4* sx = reinterpret_cast<f32x4*>(smem_all) + (size_t)rw * DB * 4 * 64 + lane;
     const int me = rw * 64 + lane;
-    for (int from = 1; from < KG; ++from) {
-      if (kg == from) {
+    __syncthreads();
+    if (kg == 1) {
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4)
-            sx[(db * 4 + r4) * 64] = f32x4{o[db][4 * r4], o[db][4 * r4 + 1], o[db][4 * r4 + 2], o[db][4 * r4 + 3]};
-        xm[me] = m_i;
-        xl[me] = l_i;
-      }
-      __syncthreads();
-      if (kg == 0) {
-        const float m1 = xm[me], m = fmaxf(m_i, m1);
-        const float a0 = m_i == m ? 1.f : fast_exp2(m_i - m), a1 = m1 == m ? 1.f : fast_exp2(m1 - m);
-        m_i = m;
-        l_i = l_i * a0 + xl[me] * a1;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const f32x4 x = sx[(db * 4 + r4) * 64];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[db][4 * r4 + e] = o[db][4 * r4 + e] * a0 + x[e] * a1;
-          }
-      }
-      __syncthreads();
+        for (int r4 = 0; r4 < 4; ++r4)
+          sx[(db * 4 + r4) * 64] = f32x4{o[db][4 * r4], o[db][4 * r4 + 1], o[db][4 * r4 + 2], o[db][4 * r4 + 3]};
+      xm[me] = m_i;
+      xl[me] = l_i;
     }
+    __syncthreads();
     if (kg != 0) return;
+    const float m1 = xm[me], m = fmaxf(m_i, m1);
+    const float a0 = m_i == m ? 1.f : fast_exp2(m_i - m), a1 = m1 == m ? 1.f : fast_exp2(m1 - m);
+    m_i = m;
+    l_i = l_i * a0 + xl[me] * a1;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x4 x = sx[(db * 4 + r4) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[db][4 * r4 + e] = o[db][4 * r4 + e] * a0 + x[e] * a1;
+      }
   }
-  if (r0 + c >= R) return;
+  // Where the second launch finds the sequence's sums.
+  if (p.part != nullptr && ck.chunk == 0 && kv == 0 && r0 == 0 && lane == 0) {
+    int* head = reinterpret_cast<int*>(p.part) + 2 * s;
+    head[0] = item;
+    head[1] = ck.count;
+  }
   const float l = l_i + __shfl_xor(l_i, 32, 64);
-  if (p.splits == 1) {
+  if (r0 + c >= R) return;
+  if (ck.count <= 1) {
     const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key: 0
     bits16* out = p.o + (((size_t)s * p.n + qi) * p.Hq + hq) * N + 4 * h;
 #pragma unroll
@@ -289,7 +426,7 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
       }
     return;
   }
-  float* part = p.part + (((size_t)blockIdx.x * p.splits + split) * R + r) * (N + 4);
+  float* part = p.part + tree_head_floats(cc.seqs) + (((size_t)item * cc.Hkv + kv) * R + r) * (N + 4);
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -300,102 +437,127 @@ __global__ __launch_bounds__((64 * Shape<N, RW>::WAVES), 1) void tree_attn_kerne
   if (h == 0) *reinterpret_cast<f32x4*>(part + N) = f32x4{m_i, l, 0.f, 0.f};
 }
 
-// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the splits, N / 4 lanes per
-// query row. Splits without a key have m = -inf and l = 0; a row without any: 0.
-template <class E, int N>
+// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a sequence's chunks, N / 4
+// lanes a row. COOP, for few rows: one workgroup a row, 1024 / N chunks at a time,
+// whose sums meet in LDS; else a row for each N / 4 lanes. Chunks without a key have
+// m = -inf and l = 0; a row without any: 0.
+template <class E, int N, bool COOP>
 __global__ __launch_bounds__(256) void tree_combine_kernel(TreeParams p) {
-  constexpr int L = N / 4;  // lanes per row
-  const int G = p.Hq / p.c.Hkv, R = p.n * G;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / L;
-  if (row >= (int64_t)p.c.seqs * p.c.Hkv * R) return;
-  const int d = (int)(id % L) * 4;
-  const int64_t bh = row / R;
-  const int r = (int)(row - bh * R), s = (int)(bh / p.c.Hkv), kv = (int)(bh - (int64_t)s * p.c.Hkv);
-  const float* part = p.part + ((size_t)bh * p.splits * R + r) * (N + 4);
-  const size_t pitch = (size_t)R * (N + 4);
+  constexpr int L = N / 4, GR = 256 / L;
+  __shared__ __attribute__((aligned(16))) float num_s[COOP ? GR : 1][COOP ? N : 4];
+  __shared__ float den_s[GR];
+  const int G = p.Hq / p.c.Hkv, R = p.n * G, tid = threadIdx.x, gi = tid / L, d = tid % L * 4;
+  const int s = blockIdx.x, row = COOP ? blockIdx.y : blockIdx.y * GR + gi;  // row: kv * R + r
+  const int* head = reinterpret_cast<const int*>(p.part) + 2 * s;
+  const int item = head[0], count = head[1];
+  if (count <= 1 || row >= p.c.Hkv * R) return;  // written by the first launch (COOP: uniform)
+  const size_t pitch = (size_t)p.c.Hkv * R * (N + 4);
+  const float* part = p.part + tree_head_floats(p.c.seqs) + ((size_t)item * p.c.Hkv * R + row) * (N + 4);
   float M = -INFINITY;
-  for (int i = 0; i < p.splits; ++i) M = fmaxf(M, part[i * pitch + N]);
+  for (int i = tid % L; i < count; i += L) M = fmaxf(M, part[i * pitch + N]);
+#pragma unroll
+  for (int off = 1; off < L; off <<= 1) M = fmaxf(M, shfl_xor(M, off));
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
   float den = 0.f;
-  for (int i = 0; i < p.splits; ++i) {
+#pragma unroll 8
+  for (int i = COOP ? gi : 0; i < count; i += COOP ? GR : 1) {
     const float* ps = part + i * pitch;
-    const float m = ps[N], w = m == M ? 1.f : exp2f(m - M);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(ps + d);
-    if (ps[N + 1] == 0.f) continue;  // (0 weights and no keys: nothing to add)
-    den = __builtin_fmaf(w, ps[N + 1], den);
+    const f32x4 ml = *reinterpret_cast<const f32x4*>(ps + N), x = *reinterpret_cast<const f32x4*>(ps + d);
+    // (A chunk without weights holds zeros: its weight is made 0, not exp2(-inf + inf).)
+    const float w = ml[1] == 0.f ? 0.f : ml[0] == M ? 1.f : exp2f(ml[0] - M);
+    den = __builtin_fmaf(w, ml[1], den);
 #pragma unroll
     for (int e = 0; e < 4; ++e) num[e] = __builtin_fmaf(w, x[e], num[e]);
   }
+  if (COOP) {
+    *reinterpret_cast<f32x4*>(&num_s[gi][d]) = num;
+    if (d == 0) den_s[gi] = den;
+    __syncthreads();
+    if (gi != 0) return;
+#pragma unroll
+    for (int g = 1; g < GR; ++g) {
+      num += *reinterpret_cast<const f32x4*>(&num_s[g][d]);
+      den += den_s[g];
+    }
+  }
   const float inv = den == 0.f ? 0.f : 1.0f / den;
-  const int qi = r / G;
+  const int kv = row / R, r = row - kv * R, qi = r / G;
   *reinterpret_cast<u32x2*>(p.o + (((size_t)s * p.n + qi) * p.Hq + kv * G + (r - qi * G)) * N + d) =
       u32x2{E::pack(num[0] * inv, num[1] * inv), E::pack(num[2] * inv, num[3] * inv)};
 }
 
-template <class E, int N>
-void launch_tree(const TreeParams& p, hipStream_t s) {
-  const int R = p.n * (p.Hq / p.c.Hkv), blocks = (R + 31) / 32;
-  const dim3 grid(p.c.seqs * p.c.Hkv, p.splits);
-  auto go = [&](auto rw) {
-    constexpr int RW = decltype(rw)::value;
-    hipLaunchKernelGGL((tree_attn_kernel<E, N, RW>), dim3(grid.x, grid.y, (blocks + RW - 1) / RW),
-                       dim3(64 * Shape<N, RW>::WAVES), 0, s, p);
-  };
-  if (blocks == 1)
-    go(std::integral_constant<int, 1>{});
-  else if (blocks == 2 || N == 256)
-    go(std::integral_constant<int, 2>{});
-  else if constexpr (N < 256)
-    go(std::integral_constant<int, 4>{});
+template <class F>
+void by_width(int N, F k) {
+  if (N == 32) k(std::integral_constant<int, 32>{});
+  if (N == 64) k(std::integral_constant<int, 64>{});
+  if (N == 128) k(std::integral_constant<int, 128>{});
+  if (N == 256) k(std::integral_constant<int, 256>{});
 }
 
 template <class E>
-hipError_t launch_tree_n(const TreeParams& p, hipStream_t s) {
-  switch (p.c.N) {
-    case 32: launch_tree<E, 32>(p, s); break;
-    case 64: launch_tree<E, 64>(p, s); break;
-    case 128: launch_tree<E, 128>(p, s); break;
-    case 256: launch_tree<E, 256>(p, s); break;
-    default: return hipErrorInvalidValue;
-  }
+hipError_t launch_tree(const TreeParams& p, hipStream_t s) {
+  by_width(p.c.N, [&](auto n) {
+    constexpr int N = decltype(n)::value;
+    const TreeGrid g = tree_grid(p.c.seqs, p.c.Hkv, p.n * (p.Hq / p.c.Hkv), p.c.max_pages << p.c.lg_page, N);
+    const dim3 grid((unsigned)(g.items * g.row_groups * p.c.Hkv));
+    if (g.blocks == 1)
+      hipLaunchKernelGGL((tree_attn_kernel<E, N, 1>), grid, dim3((64 * Tile<N, 1>::WAVES)), 0, s, p);
+    else if (g.blocks == 2)
+      hipLaunchKernelGGL((tree_attn_kernel<E, N, 2>), grid, dim3((64 * Tile<N, 2>::WAVES)), 0, s, p);
+    else
+      hipLaunchKernelGGL((tree_attn_kernel<E, N, 4>), grid, dim3((64 * Tile<N, 4>::WAVES)), 0, s, p);
+  });
   return hipGetLastError();
 }
 
 template <class E>
-hipError_t launch_combine_n(const TreeParams& p, hipStream_t s) {
-  const int64_t rows = (int64_t)p.c.seqs * p.n * p.Hq;
-  const dim3 grid((unsigned)((rows * (p.c.N / 4) + 255) / 256));
-  switch (p.c.N) {
-    case 32: hipLaunchKernelGGL((tree_combine_kernel<E, 32>), grid, dim3(256), 0, s, p); break;
-    case 64: hipLaunchKernelGGL((tree_combine_kernel<E, 64>), grid, dim3(256), 0, s, p); break;
-    case 128: hipLaunchKernelGGL((tree_combine_kernel<E, 128>), grid, dim3(256), 0, s, p); break;
-    case 256: hipLaunchKernelGGL((tree_combine_kernel<E, 256>), grid, dim3(256), 0, s, p); break;
-    default: return hipErrorInvalidValue;
-  }
+hipError_t launch_combine(const TreeParams& p, hipStream_t s) {
+  const int rows = p.n * p.Hq;
+  by_width(p.c.N, [&](auto n) {
+    constexpr int N = decltype(n)::value, GR = 1024 / N;
+    // A workgroup a row while that leaves them few (1024 rows: 8.1 us so, 9.9 with a
+    // row for each 32 lanes; 8192 rows: 24.1 / 6.9 us, N = 128).
+    if ((int64_t)p.c.seqs * rows <= 2048)
+      hipLaunchKernelGGL((tree_combine_kernel<E, N, true>), dim3(p.c.seqs, rows), dim3(256), 0, s, p);
+    else
+      hipLaunchKernelGGL((tree_combine_kernel<E, N, false>), dim3(p.c.seqs, (rows + GR - 1) / GR), dim3(256), 0, s, p);
+  });
   return hipGetLastError();
+}
+
+template <int N>
+int turn_of(int blocks) {
+  return blocks == 1 ? Tile<N, 1>::TURN : blocks == 2 ? Tile<N, 2>::TURN : Tile<N, 4>::TURN;
 }
 
 }  // namespace
 
-// Splits of a sequence's keys: as many workgroups as fill the card twice, as far
-// as the capacity gives each two tiles; and enough that a split's table fits LDS.
-int tree_splits(int seqs, int Hkv, int rows, int capacity, int N) {
-  const int blocks = (rows + 31) / 32, rw = blocks == 1 ? 1 : blocks == 2 || N == 256 ? 2 : 4;
-  const int bk = N == 256 ? 64 : rw == 1 ? 128 : 64;
-  const int64_t wgs = (int64_t)seqs * Hkv * ((blocks + rw - 1) / rw);
-  const int64_t tiles = (capacity + bk - 1) / bk;
-  int64_t s = (512 + wgs - 1) / wgs;
-  if (s > (tiles + 1) / 2) s = (tiles + 1) / 2;
-  const int64_t least = (capacity + kMaxSplitKeys - bk - 1) / (kMaxSplitKeys - bk);
-  if (s < least) s = least;
-  return s < 1 ? 1 : (int)s;
+// blocks: waves of 32 query rows that share a workgroup's tiles; want: chunks of a
+// head that run at one time; items: a bound of a head's chunks.
+TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
+  TreeGrid g;
+  const int need = (rows + 31) / 32;
+  g.blocks = need <= 2 ? need : 4;
+  g.row_groups = (need + g.blocks - 1) / g.blocks;
+  g.turn = N == 32 ? turn_of<32>(g.blocks) : N == 64 ? turn_of<64>(g.blocks) : N == 128 ? turn_of<128>(g.blocks) : turn_of<256>(g.blocks);
+  const int64_t lanes = (int64_t)Hkv * g.row_groups;
+  g.want = (int)(kSlots / lanes > 1 ? kSlots / lanes : 1);
+  // At most `want` chunks (or one per sequence) unless the largest chunk is too
+  // small; no more than the capacity has of the smallest.
+  const int64_t full = (int64_t)seqs * ((capacity + kMaxChunk - 1) / kMaxChunk);
+  const int64_t most = (int64_t)seqs * ((capacity + 2 * g.turn - 1) / (2 * g.turn));
+  g.items = g.want > seqs ? g.want : seqs;
+  if (g.items < full) g.items = full;
+  if (g.items > most) g.items = most;
+  g.split = capacity > 2 * g.turn;
+  return g;
 }
 
 hipError_t launch_tree_attn(const TreeParams& p, bool fp16, hipStream_t s) {
-  return fp16 ? launch_tree_n<Fp16>(p, s) : launch_tree_n<Bf16>(p, s);
+  return fp16 ? launch_tree<Fp16>(p, s) : launch_tree<Bf16>(p, s);
 }
 hipError_t launch_tree_combine(const TreeParams& p, bool fp16, hipStream_t s) {
-  return fp16 ? launch_combine_n<Fp16>(p, s) : launch_combine_n<Bf16>(p, s);
+  return fp16 ? launch_combine<Fp16>(p, s) : launch_combine<Bf16>(p, s);
 }
 
 }  // namespace mea
