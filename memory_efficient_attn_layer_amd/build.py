@@ -43,7 +43,8 @@ HIPCC_FLAGS = [
 # register files in the main loop (232 moves; none with VGPR accumulators). tree:
 # one wave per SIMD, likewise.
 SOURCE_FLAGS = {"tilegemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-                "tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+                "tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "grouped.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _hipcc() -> str:

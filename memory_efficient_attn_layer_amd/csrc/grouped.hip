@@ -136,8 +136,8 @@ struct TileLoad {
 // norm, with the rest 2.8e-3, with delta exact 2.5e-3).
 // ---------------------------------------------------------------------------
 template <class E, int N, bool SAVE>
-__global__ __launch_bounds__(256, N <= 64 ? 4 : N == 128 ? 3 : 1) void grouped_fwd_kernel(GroupedParams p) {
-  constexpr int BKV = N == 128 ? 32 : 64;  // keys per LDS tile
+__global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_fwd_kernel(GroupedParams p) {
+  constexpr int BKV = 64;  // keys per LDS tile
   constexpr int CH = N / 8, KS = N / 16, DB = N / 32;
   constexpr int TILE = BKV * N;
   constexpr int OP = N + 8;  // output staging pitch
