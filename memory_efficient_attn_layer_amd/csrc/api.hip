@@ -173,7 +173,7 @@ const char* const kKernelNames[K_COUNT] = {
     "qkvg_proj", "attn_fwd", "gate_oproj", "prep", "dz_gate_bwd",
     "attn_bwd_dq", "attn_bwd_dkdv", "dw_partial", "dw_reduce", "dx",
     "attn_decode", "attn_decode_combine", "skinny_gemm", "table_grad", "table_rows",
-    "grouped_fwd", "grouped_delta", "grouped_dq", "grouped_dkdv", "tree_attn", "tree_combine",
+    "grouped_fwd", "grouped_dq", "grouped_dkdv", "grouped_dkdv_join", "tree_attn", "tree_combine",
     "paged_append_plan", "paged_append_rows", "paged_accept_plan", "paged_accept_rows", "paged_truncate",
     "paged_fork_read", "paged_fork_write", "paged_compact_plan", "paged_compact_move"};
 

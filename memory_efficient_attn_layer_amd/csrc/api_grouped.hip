@@ -54,7 +54,7 @@ int check_grouped(const mea_grouped* d) {
   if (d->Hq % d->Hkv != 0) return MEA_ERR_HEADS;
   // Virtual blocks (at most total / 32 + nseq + 2 of them) times heads are the grid.
   if (d->total >= (INT64_C(1) << 30) || d->nseq >= (INT64_C(1) << 24) || d->Hq >= 65536 ||
-      (d->total / 32 + d->nseq + 2) * d->Hq >= kInt31 || d->total * d->Hq * (d->N / 8) / 256 + 1 >= kInt31)
+      (d->total / 32 + d->nseq + 2) * d->Hq >= kInt31)
     return MEA_ERR_SHAPE;
   if (!dtype_ok(d->dtype)) return MEA_ERR_DTYPE;
   if (!scale_ok(d->scale)) return MEA_ERR_SCALE;
@@ -84,6 +84,8 @@ mea::GroupedParams grouped_params(const mea_grouped* d, const void* q, const voi
   p.sl2e = d->scale * 1.4426950408889634f;
   return p;
 }
+
+size_t grouped_delta_bytes(const mea_grouped* d) { return align_up((size_t)(d->total * d->Hq) * sizeof(float)); }
 
 int check_cache(const mea_paged* c) {
   if (c == nullptr) return MEA_ERR_NULL;
@@ -179,7 +181,8 @@ int mea_grouped_fwd(const mea_grouped* d, const int32_t* cu_seqlens, const void*
 
 size_t mea_grouped_workspace_bytes(const mea_grouped* d) {
   if (check_grouped(d) != MEA_OK) return 0;
-  return align_up((size_t)d->total * (size_t)d->Hq * sizeof(float));
+  const size_t parts = (size_t)mea::dkdv_parts((int)d->total, (int)d->nseq, (int)d->Hq, (int)d->Hkv, (int)d->N);
+  return grouped_delta_bytes(d) + (parts > 1 ? align_up(parts * 2 * (size_t)(d->total * d->Hkv * d->N) * sizeof(float)) : 0);
 }
 
 int mea_grouped_bwd(const mea_grouped* d, const int32_t* cu_seqlens, const void* dout, const void* q, const void* k,
@@ -196,16 +199,17 @@ int mea_grouped_bwd(const mea_grouped* d, const int32_t* cu_seqlens, const void*
   p.o_rest = const_cast<bits16*>(static_cast<const bits16*>(o_rest));
   p.dO = static_cast<const bits16*>(dout);
   p.lse_in = lse;
-  float* delta = static_cast<float*>(ws);
-  p.delta = delta;
+  p.delta = static_cast<float*>(ws);
+  p.parts = mea::dkdv_parts(p.total, p.nseq, p.Hq, p.Hkv, (int)d->N);
+  p.sums = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + grouped_delta_bytes(d));
   p.dq = static_cast<bits16*>(dq);
   p.dk = static_cast<bits16*>(dk);
   p.dv = static_cast<bits16*>(dv);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int N = (int)d->N;
-  MEA_TRY(timed(K_GROUPED_DELTA, s, [&] { return mea::launch_grouped_delta(p, delta, N, s); }));
-  MEA_TRY(timed(K_GROUPED_DKDV, s, [&] { return mea::launch_grouped_dkdv(p, N, s); }));
   MEA_TRY(timed(K_GROUPED_DQ, s, [&] { return mea::launch_grouped_dq(p, N, s); }));
+  MEA_TRY(timed(K_GROUPED_DKDV, s, [&] { return mea::launch_grouped_dkdv(p, N, s); }));
+  if (p.parts > 1) MEA_TRY(timed(K_GROUPED_JOIN, s, [&] { return mea::launch_grouped_join(p, N, s); }));
   return MEA_OK;
 }
 

@@ -23,13 +23,17 @@ struct GroupedParams {
   float* lse;      // (Hq, total)
   // backward
   const bits16* dO;                                     // (total, Hq, N)
-  const float *lse_in, *delta;                          // (Hq, total)
+  const float* lse_in;                                  // (Hq, total)
+  float* delta;                                         // (Hq, total), from dq for dk and dv
   bits16 *dq, *dk, *dv;                                 // (total, Hq | Hkv, N)
+  int parts;    // of the dk/dv sums (dkdv_parts)
+  float* sums;  // (parts, 2, total, Hkv, N) where parts > 1
 };
+int dkdv_parts(int total, int nseq, int Hq, int Hkv, int N);
 hipError_t launch_grouped_fwd(const GroupedParams& p, int N, bool fp16, hipStream_t s);
-hipError_t launch_grouped_delta(const GroupedParams& p, float* delta, int N, hipStream_t s);
 hipError_t launch_grouped_dq(const GroupedParams& p, int N, hipStream_t s);
 hipError_t launch_grouped_dkdv(const GroupedParams& p, int N, hipStream_t s);
+hipError_t launch_grouped_join(const GroupedParams& p, int N, hipStream_t s);
 
 // A cache of fixed-size pages. Sequence s holds rows 0 .. lengths[s]-1; row r is
 // row r % page of page table[s][r / page] of both pools. refs counts the table

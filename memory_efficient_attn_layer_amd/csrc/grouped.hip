@@ -347,30 +347,11 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_f
 }
 
 // ---------------------------------------------------------------------------
-// delta (Hq, total): N / 8 lanes per (token, head) row, heads of a token next to
-// each other.
-// ---------------------------------------------------------------------------
-template <int N>
-__global__ __launch_bounds__(256) void grouped_delta_kernel(GroupedParams p, float* delta) {
-  constexpr int CH = N / 8;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / CH;
-  const bool in = row < (int64_t)p.total * p.Hq;
-  float a[8], b[8], r[8], d = 0.f;
-  const size_t at = in ? (size_t)id * 8 : 0;
-  unpack8(ld16(p.dO + at), a);
-  unpack8(ld16(p.o + at), b);
-  unpack8(ld16(p.o_rest + at), r);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) d = __builtin_fmaf(a[e], b[e] + r[e], d);
-#pragma unroll
-  for (int off = 1; off < CH; off <<= 1) d += shfl_xor(d, off);
-  if (in && id % CH == 0) delta[(size_t)(row % p.Hq) * p.total + row / p.Hq] = d;
-}
-
-// ---------------------------------------------------------------------------
 // dQ: the forward's work list and key tiles. S^T = K Q^T and dP^T = V dO^T, the
 // accumulators of the latter starting from -delta (four copies of each query's
-// in LDS, read into the registers), dQ^T += K^T dS^T.
+// in LDS, read into the registers), dQ^T += K^T dS^T. delta is formed here, from the
+// dO rows that are held anyway, and left for the dK/dV kernel (a launch of its own
+// for it took 13 us at 26000 tokens, 8 heads of 64, 26 at 16384, 16 of 128).
 //
 // A sequence's first query sees one key, whose weight is 1 whatever the score:
 // its ds is 0, set so rather than left to the difference of two roundings.
@@ -419,7 +400,22 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 256 ? 1 : 2) void grouped_d
   const float nl = -p.lse_in[(size_t)head * p.total + tq] * kLog2e;
   f32x4* stat = reinterpret_cast<f32x4*>(smem_raw + SM_LOOP) + wave * 128;
   {
-    const float nd = -p.delta[(size_t)head * p.total + tq];
+    // This lane has half of the row; the other half is lane ^ 32's.
+    const bits16* orow = p.o + ((size_t)tq * p.Hq + head) * N + 8 * h;
+    const bits16* rest = p.o_rest + ((size_t)tq * p.Hq + head) * N + 8 * h;
+    float d = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const u32x4 a = ld16(orow + 16 * ks), b = ld16(rest + 16 * ks);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d = __builtin_fmaf(E::lo(df[ks][e]), E::lo(a[e]) + E::lo(b[e]), d);
+        d = __builtin_fmaf(E::hi(df[ks][e]), E::hi(a[e]) + E::hi(b[e]), d);
+      }
+    }
+    d += __shfl_xor(d, 32, 64);
+    if (h == 0 && q0w + c < T) p.delta[(size_t)head * p.total + tq] = d;
+    const float nd = -d;
 #pragma unroll
     for (int j = 0; j < 2; ++j) stat[(2 * h + j) * 32 + c] = f32x4{nd, nd, nd, nd};
   }
@@ -535,7 +531,10 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 256 ? 1 : 2) void grouped_d
 // dK, dV: one workgroup per (segment, key head, 128 keys), wave w its keys
 // 32 w .. 32 w + 31; the query tiles of every head of the group stream through
 // LDS, so the sum over the group stays in the accumulators (fixed order, no
-// atomics). S = Q K^T and dP = dO V^T with the key on the lane; the start values
+// atomics). The tiles, head after head, are cut into p.parts equal runs for as many
+// workgroups where the key blocks alone are too few to fill the card and even out
+// the causal blocks' lengths (see dkdv_parts); their fp32 sums are then added, in
+// order, by a second launch. S = Q K^T and dP = dO V^T with the key on the lane; the start values
 // -lse / scale and -delta come from LDS rows. dV^T += dO^T P, dK^T += Q^T dS.
 // ---------------------------------------------------------------------------
 template <class E, int N>
@@ -554,11 +553,13 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_d
   float* statf = reinterpret_cast<float*>(smem + 2 * 2 * TILE * 2);        // [stage][-lse / scale | -delta][query]
   u32x4* vown = reinterpret_cast<u32x4*>(smem + SM_LOOP);
 
-  const int G = p.Hq / p.Hkv, kv = blockIdx.x % p.Hkv;
-  const Segment sg = find_segment(p.cu, p.nseq, p.total, BK, blockIdx.x / p.Hkv);
+  const int G = p.Hq / p.Hkv, kv = blockIdx.x % p.Hkv, vp = blockIdx.x / p.Hkv;
+  const int part = vp % p.parts;
+  const Segment sg = find_segment(p.cu, p.nseq, p.total, BK, vp / p.parts);
   const int T = sg.len, k0 = sg.blk * BK;
   if (k0 >= T) return;
   if (!sg.live) {
+    if (part != 0) return;
     zero_rows<N>(p.dk, sg.start + k0, sg.start + min(k0 + BK, T), kv, 1, p.Hkv);
     zero_rows<N>(p.dv, sg.start + k0, sg.start + min(k0 + BK, T), kv, 1, p.Hkv);
     return;
@@ -674,11 +675,13 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_d
   const int nq = (T - k0 + BQ - 1) / BQ, nfull = nq - BK / BQ;
   const bool ragged = (T - k0) % BQ != 0;
   auto row_of = [&](int it) { return k0 + (nq - 1 - it) * BQ; };
-  int g = 0, stage = 0;
+  // This part's run: tiles first .. last - 1 of the nq * G.
+  const int n = nq * G, first = (int)((int64_t)n * part / p.parts), last = (int)((int64_t)n * (part + 1) / p.parts);
+  int g = first / nq, left = last - first, stage = 0;
   auto tile = [&](int it, auto masked_tag) {
     constexpr bool MASKED = decltype(masked_tag)::value;
     const int q0 = row_of(it);
-    const bool wrap = it + 1 == nq, more = !wrap || g + 1 < G;
+    const bool wrap = it + 1 == nq, more = --left > 0;
     if (more) issue_tile(kv * G + g + (wrap ? 1 : 0), row_of(wrap ? 0 : it + 1), stage ^ 1);
     const bits16* qt = tiles + stage * 2 * TILE;
     const bits16* dt = qt + TILE;
@@ -696,17 +699,38 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_d
     __syncthreads();
     stage ^= 1;
   };
-  issue_tile(kv * G, row_of(0), 0);
-  wait_vmcnt0();
-  publish(0);
-  __syncthreads();
-  for (; g < G; ++g) {
-    int it = 0;
-    if (nfull > 0 && ragged) tile(it++, std::true_type{});
-    for (; it < nfull; ++it) tile(it, std::false_type{});
-    for (; it < nq; ++it) tile(it, std::true_type{});
+  if (left > 0) {
+    issue_tile(kv * G + g, row_of(first - g * nq), 0);
+    wait_vmcnt0();
+    publish(0);
+    __syncthreads();
+  }
+  int it = first - g * nq;
+  while (left > 0) {
+    const int end = min(nq, it + left), full = min(nfull, end);
+    if (it == 0 && nfull > 0 && ragged) tile(it++, std::true_type{});
+    for (; it < full; ++it) tile(it, std::false_type{});
+    for (; it < end; ++it) tile(it, std::true_type{});
+    ++g;
+    it = 0;
   }
 
+  if (p.parts > 1) {
+    // fp32 sums: (part, dk | dv, token, key head, N); a lane has 4 columns at a time.
+    float* out = p.sums + (((size_t)part * 2 * p.total + sg.start + kw0 + c) * p.Hkv + kv) * N + 4 * h;
+    if (kw0 + c < T) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          float* at = out + 32 * db + 8 * r4;
+          *reinterpret_cast<f32x4*>(at) = f32x4{dk[db][4 * r4], dk[db][4 * r4 + 1], dk[db][4 * r4 + 2], dk[db][4 * r4 + 3]};
+          *reinterpret_cast<f32x4*>(at + (size_t)p.total * p.Hkv * N) =
+              f32x4{dv[db][4 * r4], dv[db][4 * r4 + 1], dv[db][4 * r4 + 2], dv[db][4 * r4 + 3]};
+        }
+    }
+    return;
+  }
   bits16* stg = reinterpret_cast<bits16*>(smem) + wave * 32 * OP;
   auto store = [&](const f32x16 (&a)[DB], float f, bits16* out) {
 #pragma unroll
@@ -727,6 +751,28 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_d
   };
   store(dv, 1.0f, p.dv);
   store(dk, p.scale, p.dk);
+}
+
+// The sums of the parts, eight elements a thread, to dk (times scale) and dv. Rows
+// of no sequence have no sums: they stay as the first launch zeroed them.
+template <class E>
+__global__ __launch_bounds__(256) void grouped_dkdv_join_kernel(GroupedParams p, int N) {
+  const size_t each = (size_t)p.total * p.Hkv * N, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at >= each) return;
+  const int t = (int)(at / ((size_t)p.Hkv * N));
+  if (t < p.cu[0] || t >= p.cu[p.nseq]) return;
+  f32x4 a[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = zero4();
+  for (int part = 0; part < p.parts; ++part) {
+    const float* s = p.sums + (size_t)part * 2 * each + at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] += *reinterpret_cast<const f32x4*>(s + (i >> 1) * each + (i & 1) * 4);
+  }
+  a[0] *= p.scale;
+  a[1] *= p.scale;
+  st16(p.dk + at, u32x4{E::pack(a[0][0], a[0][1]), E::pack(a[0][2], a[0][3]), E::pack(a[1][0], a[1][1]), E::pack(a[1][2], a[1][3])});
+  st16(p.dv + at, u32x4{E::pack(a[2][0], a[2][1]), E::pack(a[2][2], a[2][3]), E::pack(a[3][0], a[3][1]), E::pack(a[3][2], a[3][3])});
 }
 
 // Calls k(std::integral_constant<int, N>) for a supported head width.
@@ -752,6 +798,27 @@ unsigned query_grid(const GroupedParams& p) {
 
 }  // namespace
 
+// Parts of a key block's query tiles, at most eight: as many as fill the card, with
+// four tiles each at least; or as many as give its slots four workgroups each, which
+// evens out the causal blocks' lengths, where a part has 64 tiles at least, whose
+// time makes up for the sums' way through memory. (T = 8192 x 2, 16 / 4 heads of 128,
+// 1 / 4 parts: dK/dV with the join 1394 / 864 us; 24 sequences of 1100 on average, 8 /
+// 4 heads of 64, 17 tiles a block: 147 / 199 us.)
+int dkdv_parts(int total, int nseq, int Hq, int Hkv, int N) {
+  const int64_t slots = 256 * (N <= 64 ? 3 : N == 128 ? 2 : 1), blocks = (int64_t)(total / 128 + nseq) * Hkv;
+  const int64_t tiles = (int64_t)(total / nseq) * (Hq / Hkv) / (2 * (N >= 128 ? 32 : 64));  // of a block, on average
+  const int64_t fill = slots / blocks < tiles / 4 ? slots / blocks : tiles / 4;
+  const int64_t even = (4 * slots + blocks - 1) / blocks, parts = even < tiles / 64 ? even : tiles / 64;
+  const int64_t n = fill > parts ? fill : parts;
+  return n < 1 ? 1 : n > 8 ? 8 : (int)n;
+}
+
+hipError_t launch_grouped_join(const GroupedParams& p, int N, hipStream_t s) {
+  const size_t threads = (size_t)p.total * p.Hkv * N / 8;
+  hipLaunchKernelGGL(grouped_dkdv_join_kernel<Bf16>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p, N);
+  return hipGetLastError();
+}
+
 hipError_t launch_grouped_fwd(const GroupedParams& p, int N, bool fp16, hipStream_t s) {
   const dim3 grid(query_grid(p));
   return by_width(N, [&](auto n) {
@@ -764,19 +831,13 @@ hipError_t launch_grouped_fwd(const GroupedParams& p, int N, bool fp16, hipStrea
   });
 }
 
-hipError_t launch_grouped_delta(const GroupedParams& p, float* delta, int N, hipStream_t s) {
-  const int64_t threads = (int64_t)p.total * p.Hq * (N / 8);
-  const dim3 grid((unsigned)((threads + 255) / 256));
-  return by_width(N, [&](auto n) { hipLaunchKernelGGL((grouped_delta_kernel<n.value>), grid, dim3(256), 0, s, p, delta); });
-}
-
 hipError_t launch_grouped_dq(const GroupedParams& p, int N, hipStream_t s) {
   const dim3 grid(query_grid(p));
   return by_width(N, [&](auto n) { hipLaunchKernelGGL((grouped_dq_kernel<Bf16, n.value>), grid, dim3(256), 0, s, p); });
 }
 
 hipError_t launch_grouped_dkdv(const GroupedParams& p, int N, hipStream_t s) {
-  const dim3 grid((unsigned)virtual_blocks(p.total, p.nseq, 128) * (unsigned)p.Hkv);
+  const dim3 grid((unsigned)virtual_blocks(p.total, p.nseq, 128) * (unsigned)(p.Hkv * p.parts));
   return by_width(N, [&](auto n) { hipLaunchKernelGGL((grouped_dkdv_kernel<Bf16, n.value>), grid, dim3(256), 0, s, p); });
 }
 

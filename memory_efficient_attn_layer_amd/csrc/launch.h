@@ -10,7 +10,7 @@ enum KernelId {
   K_QKVG_PROJ, K_ATTN_FWD, K_GATE_OPROJ, K_PREP, K_DZ_GATE_BWD,
   K_ATTN_BWD_DQ, K_ATTN_BWD_DKDV, K_DW_PARTIAL, K_DW_REDUCE, K_DX,
   K_ATTN_DECODE, K_DECODE_COMBINE, K_SKINNY_GEMM, K_TABLE_GRAD, K_TABLE_ROWS,
-  K_GROUPED_FWD, K_GROUPED_DELTA, K_GROUPED_DQ, K_GROUPED_DKDV, K_TREE_ATTN, K_TREE_COMBINE,
+  K_GROUPED_FWD, K_GROUPED_DQ, K_GROUPED_DKDV, K_GROUPED_JOIN, K_TREE_ATTN, K_TREE_COMBINE,
   K_APPEND_PLAN, K_APPEND_ROWS, K_ACCEPT_PLAN, K_ACCEPT_ROWS, K_TRUNCATE,
   K_FORK_READ, K_FORK_WRITE, K_COMPACT_PLAN, K_COMPACT_MOVE, K_COUNT
 };
