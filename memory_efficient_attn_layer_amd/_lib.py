@@ -137,6 +137,8 @@ def _check_single_hip_runtime() -> None:
 def load() -> ctypes.CDLL:
     """Loads (once) and returns the library; raises if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -194,7 +196,7 @@ _same_device = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """A context with ``device`` current (nothing to do where it is already)."""
-    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _same_device if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -205,6 +207,18 @@ def stream_of(device: torch.device) -> int:
     """The current stream's handle (without building a Stream object)."""
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+@functools.lru_cache(maxsize=512)
+def grouped_desc(*values) -> MeaGrouped:
+    """A mea_grouped of these values (the library only reads it)."""
+    return MeaGrouped(*values)
+
+
+@functools.lru_cache(maxsize=512)
+def strides(*values) -> ctypes.Array:
+    """An int64 array of these values (the library only reads it)."""
+    return (ctypes.c_int64 * len(values))(*values)
 
 
 def profile_enable(on: bool) -> None:

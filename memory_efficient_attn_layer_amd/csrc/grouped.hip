@@ -808,7 +808,7 @@ int dkdv_parts(int total, int nseq, int Hq, int Hkv, int N) {
   const int64_t slots = 256 * (N <= 64 ? 3 : N == 128 ? 2 : 1), blocks = (int64_t)(total / 128 + nseq) * Hkv;
   const int64_t tiles = (int64_t)(total / nseq) * (Hq / Hkv) / (2 * (N >= 128 ? 32 : 64));  // of a block, on average
   const int64_t fill = slots / blocks < tiles / 4 ? slots / blocks : tiles / 4;
-  const int64_t even = (4 * slots + blocks - 1) / blocks, parts = even < tiles / 64 ? even : tiles / 64;
+  const int64_t even = (3 * slots + blocks - 1) / blocks, parts = even < tiles / 64 ? even : tiles / 64;
   const int64_t n = fill > parts ? fill : parts;
   return n < 1 ? 1 : n > 8 ? 8 : (int)n;
 }

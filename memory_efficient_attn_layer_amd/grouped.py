@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _lib
-from .attention import _wants_grad, check_offsets
+from .attention import check_offsets
 
 SUPPORTED_WIDTHS = (32, 64, 128, 256)
 MAX_TOKEN_STRIDE = 1 << 24  # elements
@@ -34,13 +34,19 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _rows(t: torch.Tensor, limit: int = MAX_TOKEN_STRIDE) -> torch.Tensor:
-    """``t`` (..., N) as the library reads it, with any strides that are
-    multiples of 8 elements (the token's, second to last but one, up to
-    ``limit``); a dense copy of anything else."""
-    st = t.stride()
-    ok = st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 0 for s in st[:-1]) and st[-3] <= limit
-    return t if ok else _aligned(t)
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (.., tokens, heads, N) as the library reads it, with any strides that
+    are multiples of 8 elements; a dense copy of anything else."""
+    *outer, last = t.stride()
+    bits = t.data_ptr() >> 1
+    for s in outer:
+        bits |= s
+    return t if last == 1 and bits & 7 == 0 else _aligned(t)
+
+
+def _tokens(t: torch.Tensor) -> torch.Tensor:
+    """The same for (tokens, heads, N), whose token stride has a limit."""
+    return _rows(t) if t.stride(0) <= MAX_TOKEN_STRIDE else _aligned(t)
 
 
 def _validate(q, k, v) -> None:
@@ -68,31 +74,39 @@ def _validate(q, k, v) -> None:
 
 
 def _desc(q, k, v, nseq: int, scale: float) -> _lib.MeaGrouped:
-    return _lib.MeaGrouped(q.shape[0], nseq, q.shape[1], k.shape[1], q.shape[2], q.stride(0), q.stride(1), k.stride(0),
-                           k.stride(1), v.stride(0), v.stride(1), scale, _lib.MEA_DTYPES[q.dtype])
+    total, Hq, N = q.shape
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    return _lib.grouped_desc(total, nseq, Hq, k.shape[1], N, sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], scale,
+                             _lib.MEA_DTYPES[q.dtype])
+
+
+def _forward(q, k, v, cu_seqlens, scale, save):
+    """(o, o_rest, lse), the last two None without ``save``; q, k, v as _tokens leaves them."""
+    dev = q.device
+    d = _desc(q, k, v, cu_seqlens.shape[0] - 1, scale)
+    total, Hq, N = q.shape
+    o = torch.empty((total, Hq, N), device=dev, dtype=q.dtype)
+    rest = torch.empty_like(o) if save else None
+    lse = torch.empty((Hq, total), device=dev, dtype=torch.float32) if save else None
+    with _lib.on_device(dev):
+        rc = _lib.load().mea_grouped_fwd(d, cu_seqlens.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                         _lib.ptr(rest), _lib.ptr(lse), _lib.stream_of(dev))
+    if rc != 0:
+        _lib.check(rc, "mea_grouped_fwd")
+    return o, rest, lse
 
 
 class GroupedAttentionFunction(torch.autograd.Function):
-    """Autograd op behind ``grouped_attn_varlen``: saves q, k, v, the output, what
-    rounding it to 16 bits left and its log-sum-exp; without a gradient requirement it saves nothing."""
+    """Autograd op behind ``grouped_attn_varlen`` where a gradient is wanted:
+    saves q, k, v, the output, what rounding it to 16 bits left and its
+    log-sum-exp."""
 
     @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, scale, save):
-        lib = _lib.load()
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        total, Hq, N = q.shape
-        dev = q.device
-        d = _desc(q, k, v, cu_seqlens.numel() - 1, scale)
-        o = torch.empty((total, Hq, N), device=dev, dtype=q.dtype)
-        rest = torch.empty_like(o) if save else None
-        lse = torch.empty((Hq, total), device=dev, dtype=torch.float32) if save else None
-        with _lib.on_device(dev):
-            rc = lib.mea_grouped_fwd(d, cu_seqlens.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                                     _lib.ptr(rest), _lib.ptr(lse), _lib.stream_of(dev))
-        _lib.check(rc, "mea_grouped_fwd")
-        if save:
-            ctx.save_for_backward(q, k, v, cu_seqlens, o, rest, lse)
-            ctx.scale = scale
+    def forward(ctx, q, k, v, cu_seqlens, scale):
+        q, k, v = _tokens(q), _tokens(k), _tokens(v)
+        o, rest, lse = _forward(q, k, v, cu_seqlens, scale, True)
+        ctx.save_for_backward(q, k, v, cu_seqlens, o, rest, lse)
+        ctx.scale = scale
         return o
 
     @staticmethod
@@ -111,7 +125,7 @@ class GroupedAttentionFunction(torch.autograd.Function):
                                      o.data_ptr(), rest.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                      ws.data_ptr(), ws_bytes, _lib.stream_of(dev))
         _lib.check(rc, "mea_grouped_bwd")
-        return dq, dk, dv, None, None, None
+        return dq, dk, dv, None, None
 
 
 def grouped_attn_varlen(q, k, v, cu_seqlens, scale=None):
@@ -130,10 +144,12 @@ def grouped_attn_varlen(q, k, v, cu_seqlens, scale=None):
         cu_seqlens = torch.tensor(host, dtype=torch.int32, device=q.device)
     elif cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.device != q.device:
         raise ValueError("cu_seqlens must be a 1-D int32 tensor of nseq + 1 offsets on the device of q")
-    save = _wants_grad(q, k, v)
-    if save and q.dtype != torch.bfloat16:
+    cu_seqlens = cu_seqlens.contiguous()
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return _forward(_tokens(q), _tokens(k), _tokens(v), cu_seqlens, scale, False)[0]
+    if q.dtype != torch.bfloat16:
         raise TypeError(f"gradients are taken in bfloat16 only, got {q.dtype}")
-    return GroupedAttentionFunction.apply(q, k, v, cu_seqlens.contiguous(), scale, save)
+    return GroupedAttentionFunction.apply(q, k, v, cu_seqlens, scale)
 
 
 __all__ = ["GroupedAttentionFunction", "grouped_attn_varlen", "SUPPORTED_WIDTHS"]

@@ -16,12 +16,11 @@ share their prompt, and a finished sequence's pages serve the next one:
 All of it runs in libmea.so on the current stream. The tables live on the GPU and
 change there in stream order: no call waits for the GPU (but ``verify`` and the
 hand-over of lists), and all of them can be captured into a graph. A cache is
-used by one stream at a time. ``tree_attn`` takes no gradient, like
+used by one stream at a time (its calls share a workspace). ``tree_attn`` takes no gradient, like
 ``decode_step``.
 """
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass, field
 
 import torch
@@ -31,14 +30,6 @@ from .grouped import SUPPORTED_WIDTHS, _check_scale, _rows
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_TREE = 256  # new tokens per sequence
-
-_NO_LIMIT = 1 << 62
-
-
-def _strides(*tensors) -> ctypes.Array:
-    st = [s for t in tensors for s in t]
-    return (ctypes.c_int64 * len(st))(*st)
-
 
 @dataclass(frozen=True, eq=False)
 class PagedKVCache:
@@ -56,7 +47,8 @@ class PagedKVCache:
     refs: torch.Tensor
     status: torch.Tensor
     _c: _lib.MeaPaged = field(init=False, repr=False)
-    _ws_bytes: int = field(init=False, repr=False)
+    _ws: torch.Tensor = field(init=False, repr=False)  # of the cache's own calls, which come one after the other
+    _tree_ws: dict = field(init=False, repr=False)  # (n, Hq) -> workspace bytes of tree_attn
 
     @classmethod
     def empty(cls, sequences: int, H: int, N: int, pages: int, device, page: int = 64, max_pages: int | None = None,
@@ -102,9 +94,11 @@ class PagedKVCache:
                           self.refs.data_ptr(), self.status.data_ptr(), S, pages, H, page, N, M,
                           _lib.MEA_DTYPES[self.k.dtype])
         object.__setattr__(self, "_c", c)
-        object.__setattr__(self, "_ws_bytes", _lib.load().mea_paged_workspace_bytes(c))
-        if self._ws_bytes == 0:
+        ws_bytes = _lib.load().mea_paged_workspace_bytes(c)
+        if ws_bytes == 0:
             raise ValueError(f"cache of {S} sequences, {pages} pages and {M} pages a sequence is out of range")
+        object.__setattr__(self, "_ws", torch.empty(ws_bytes, device=self.k.device, dtype=torch.uint8))
+        object.__setattr__(self, "_tree_ws", {})
 
     @property
     def sequences(self) -> int:
@@ -131,12 +125,11 @@ class PagedKVCache:
         self._on_gpu()
         S, (_, H, _, N) = self.sequences, self.k.shape
         packed = cu_seqlens is not None
-        want = ("total", H, N) if packed else (S, "n", H, N)
         for name, t in (("k", k), ("v", v)):
-            if not isinstance(t, torch.Tensor) or t.dim() != len(want) or t.shape != k.shape or any(
-                    isinstance(w, int) and w != x for w, x in zip(want, t.shape)):
+            if not isinstance(t, torch.Tensor) or t.shape != (
+                    (k.shape[0], H, N) if packed else (S, k.shape[1] if k.dim() > 1 else 0, H, N)):
                 shape = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__
-                raise ValueError(f"{name} must be ({', '.join(map(str, want))}), got {shape}")
+                raise ValueError(f"{name} must be ({'total' if packed else f'{S}, n'}, {H}, {N}), got {shape}")
             if t.dtype != self.k.dtype or t.device != self.k.device:
                 raise TypeError(f"{name} is {t.dtype} on {t.device}, the cache {self.k.dtype} on {self.k.device}")
         total = k.shape[0] if packed else S * k.shape[1]
@@ -144,12 +137,11 @@ class PagedKVCache:
             cu_seqlens = self._ints("cu_seqlens", cu_seqlens, S + 1, offsets=total)
         if total == 0:
             return
-        k, v = _rows(k, _NO_LIMIT), _rows(v, _NO_LIMIT)
-        st = _strides(*(((0,) + t.stride()[:2]) if packed else t.stride()[:3] for t in (k, v)))
-        ws = self._workspace()
+        k, v = _rows(k), _rows(v)
+        st = _lib.strides(0, *k.stride()[:2], 0, *v.stride()[:2]) if packed else _lib.strides(*k.stride()[:3], *v.stride()[:3])
         with _lib.on_device(k.device):
             rc = _lib.load().mea_paged_append(self._c, k.data_ptr(), v.data_ptr(), st, _lib.ptr(cu_seqlens),
-                                              0 if packed else k.shape[1], total, ws.data_ptr(), self._ws_bytes,
+                                              0 if packed else k.shape[1], total, self._ws.data_ptr(), self._ws.shape[0],
                                               _lib.stream_of(k.device))
         _lib.check(rc, "mea_paged_append")
 
@@ -169,10 +161,9 @@ class PagedKVCache:
                 or path.dtype != torch.int32 or path.device != self.k.device):
             raise ValueError(f"path must be an int32 tensor ({self.sequences}, 1 .. {n}) on {self.k.device}")
         path, counts = path.contiguous(), self._ints("counts", counts, self.sequences)
-        ws = self._workspace()
         with _lib.on_device(path.device):
             rc = _lib.load().mea_paged_accept(self._c, n, path.data_ptr(), path.shape[1], counts.data_ptr(),
-                                              ws.data_ptr(), self._ws_bytes, _lib.stream_of(path.device))
+                                              self._ws.data_ptr(), self._ws.shape[0], _lib.stream_of(path.device))
         _lib.check(rc, "mea_paged_accept")
 
     def truncate(self, lengths) -> None:
@@ -201,9 +192,8 @@ class PagedKVCache:
         device tensor or a list."""
         self._on_gpu()
         parents = self._ints("parents", parents, self.sequences)
-        ws = self._workspace()
         with _lib.on_device(parents.device):
-            rc = _lib.load().mea_paged_fork(self._c, parents.data_ptr(), ws.data_ptr(), self._ws_bytes,
+            rc = _lib.load().mea_paged_fork(self._c, parents.data_ptr(), self._ws.data_ptr(), self._ws.shape[0],
                                             _lib.stream_of(parents.device))
         _lib.check(rc, "mea_paged_fork")
 
@@ -212,9 +202,8 @@ class PagedKVCache:
         pages 0 .. (how many there are) - 1."""
         self._on_gpu()
         dev = self.k.device
-        ws = self._workspace()
         with _lib.on_device(dev):
-            rc = _lib.load().mea_paged_compact(self._c, ws.data_ptr(), self._ws_bytes, _lib.stream_of(dev))
+            rc = _lib.load().mea_paged_compact(self._c, self._ws.data_ptr(), self._ws.shape[0], _lib.stream_of(dev))
         _lib.check(rc, "mea_paged_compact")
 
     def verify(self) -> None:
@@ -231,9 +220,6 @@ class PagedKVCache:
     def _on_gpu(self) -> None:
         if not self.k.is_cuda:
             raise RuntimeError("PagedKVCache runs only on a ROCm GPU device (there is no CPU path)")
-
-    def _workspace(self) -> torch.Tensor:
-        return torch.empty(self._ws_bytes, device=self.k.device, dtype=torch.uint8)
 
     def _ints(self, name: str, values, n: int, offsets: int | None = None) -> torch.Tensor:
         """``values`` as an int32 device tensor of n entries (``offsets``: the
@@ -289,12 +275,14 @@ def tree_attn(q, cache: PagedKVCache, mask=None, scale=None) -> torch.Tensor:
     cache._on_gpu()
     lib = _lib.load()
     dev = q.device
-    q4 = _rows(q4, _NO_LIMIT)
+    q4 = _rows(q4)
     o = torch.empty((S, n, Hq, N), device=dev, dtype=q.dtype)
-    ws_bytes = lib.mea_tree_workspace_bytes(cache._c, n, Hq)
+    ws_bytes = cache._tree_ws.get((n, Hq))
+    if ws_bytes is None:
+        ws_bytes = cache._tree_ws[(n, Hq)] = lib.mea_tree_workspace_bytes(cache._c, n, Hq)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
     with _lib.on_device(dev):
-        rc = lib.mea_tree_attn(cache._c, n, Hq, scale, q4.data_ptr(), _strides(q4.stride()[:3]), _lib.ptr(mask), mask_seq,
+        rc = lib.mea_tree_attn(cache._c, n, Hq, scale, q4.data_ptr(), _lib.strides(*q4.stride()[:3]), _lib.ptr(mask), mask_seq,
                                o.data_ptr(), _lib.ptr(ws), ws_bytes, _lib.stream_of(dev))
     _lib.check(rc, "mea_tree_attn")
     return o if q.dim() == 4 else o[:, 0]
