@@ -24,10 +24,12 @@
 //
 // Work list: no host knows the lengths. The boundaries 0, cu[0], ..,
 // cu[nseq], total cut the tokens into nseq + 2 segments (the first and the last
-// hold no sequence; their outputs are zeros). Segment i owns the virtual blocks
-// from b_i / BT + i on (BT tokens a block), which leaves room for ceil(len / BT)
-// of them; a workgroup finds its segment by counting the starts at or below its
-// block, 64 at a time.
+// hold no sequence; their outputs are zeros). Up to 64 segments are taken longest
+// first, a segment's longest block first, so that the longest blocks of the call do
+// not start last: each lane of a wave holds one segment and sums up the blocks of
+// those before it. Of more segments, segment i owns the virtual blocks from
+// b_i / BT + i on (BT tokens a block), which leaves room for ceil(len / BT) of
+// them, and a workgroup counts the starts at or below its block, 64 at a time.
 #include <type_traits>
 
 #include "elem.cuh"
@@ -45,17 +47,39 @@ struct Segment {
 // Virtual blocks of BT tokens.
 __host__ __device__ inline int virtual_blocks(int total, int nseq, int BT) { return total / BT + nseq + 2; }
 
+// The v-th block of the work list. LAST: a segment's last block is its longest (a
+// block of queries), else its first (of keys).
+template <bool LAST>
 __device__ __forceinline__ Segment find_segment(const int* cu, int nseq, int total, int BT, int v) {
   const int lane = threadIdx.x & 63;
   // Boundary i: 0, cu[0] .. cu[nseq], offsets clamped to [0, total].
   auto bound = [&](int i) { return i == 0 ? 0 : i == nseq + 2 ? total : min(max(cu[i - 1], 0), total); };
+  Segment s;
+  if (nseq + 2 <= 64) {
+    const int i = min(lane, nseq + 1), start = bound(i), len = lane < nseq + 2 ? max(bound(i + 1) - start, 0) : 0;
+    const int blocks = (len + BT - 1) / BT;
+    int before = 0;  // blocks of the segments in front of this lane's
+    for (int j = 0; j < nseq + 2; ++j) {
+      const int other = __builtin_amdgcn_readlane(blocks, j);
+      before += other > blocks || (other == blocks && j < lane) ? other : 0;
+    }
+    const unsigned long long mine = __ballot(v >= before && v < before + blocks);
+    const int l = mine != 0 ? __ffsll(mine) - 1 : 63;
+    s.start = __builtin_amdgcn_readlane(start, l);
+    s.len = mine != 0 ? __builtin_amdgcn_readlane(len, l) : 0;
+    s.blk = v - __builtin_amdgcn_readlane(before, l);
+    if (LAST) s.blk = __builtin_amdgcn_readlane(blocks, l) - 1 - s.blk;
+    if (mine == 0) s.blk = 0;
+    s.live = l > 0 && l <= nseq;
+    return s;
+  }
+  if (LAST) v = virtual_blocks(total, nseq, BT) - 1 - v;
   int n = 0;
   for (int i0 = 0; i0 < nseq + 2; i0 += 64) {
     const int i = i0 + lane;
     n += __popcll(__ballot(i < nseq + 2 && bound(min(i, nseq + 1)) / BT + i <= v));
   }
   const int i = __builtin_amdgcn_readfirstlane(max(n - 1, 0));
-  Segment s;
   s.start = __builtin_amdgcn_readfirstlane(bound(i));
   s.len = max(__builtin_amdgcn_readfirstlane(bound(i + 1)) - s.start, 0);
   s.blk = v - s.start / BT - i;
@@ -148,8 +172,7 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_f
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.Hq / p.Hkv, hw = heads_per_wg(G), BT = 128 / hw, NH = p.Hq / hw;
   const HeadGroup hg = head_group(blockIdx.x % NH, p.Hkv, G, hw);
-  const int v = virtual_blocks(p.total, p.nseq, BT) - 1 - blockIdx.x / NH;
-  const Segment sg = find_segment(p.cu, p.nseq, p.total, BT, v);
+  const Segment sg = find_segment<true>(p.cu, p.nseq, p.total, BT, blockIdx.x / NH);
   const int T = sg.len, b0 = sg.blk * BT;
   if (b0 >= T) return;  // uniform, before any barrier
   if (!sg.live) {
@@ -371,8 +394,7 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 256 ? 1 : 2) void grouped_d
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.Hq / p.Hkv, hw = heads_per_wg(G), BT = 128 / hw, NH = p.Hq / hw;
   const HeadGroup hg = head_group(blockIdx.x % NH, p.Hkv, G, hw);
-  const int v = virtual_blocks(p.total, p.nseq, BT) - 1 - blockIdx.x / NH;
-  const Segment sg = find_segment(p.cu, p.nseq, p.total, BT, v);
+  const Segment sg = find_segment<true>(p.cu, p.nseq, p.total, BT, blockIdx.x / NH);
   const int T = sg.len, b0 = sg.blk * BT;
   if (b0 >= T) return;
   if (!sg.live) {
@@ -555,7 +577,7 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_d
 
   const int G = p.Hq / p.Hkv, kv = blockIdx.x % p.Hkv, vp = blockIdx.x / p.Hkv;
   const int part = vp % p.parts;
-  const Segment sg = find_segment(p.cu, p.nseq, p.total, BK, vp / p.parts);
+  const Segment sg = find_segment<false>(p.cu, p.nseq, p.total, BK, vp / p.parts);
   const int T = sg.len, k0 = sg.blk * BK;
   if (k0 >= T) return;
   if (!sg.live) {
