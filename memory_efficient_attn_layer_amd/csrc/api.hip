@@ -175,7 +175,7 @@ const char* const kKernelNames[K_COUNT] = {
     "attn_decode", "attn_decode_combine", "skinny_gemm", "table_grad", "table_rows",
     "grouped_fwd", "grouped_dq", "grouped_dkdv", "grouped_dkdv_join", "tree_attn", "tree_combine",
     "paged_append_plan", "paged_append_rows", "paged_accept_plan", "paged_accept_rows", "paged_truncate",
-    "paged_fork_read", "paged_fork_write", "paged_compact_plan", "paged_compact_move"};
+    "paged_fork", "paged_fork_read", "paged_fork_write", "paged_compact_plan", "paged_compact_move"};
 
 struct ProfRec {
   int kernel;

@@ -283,6 +283,10 @@ int mea_paged_fork(const mea_paged* c, const int32_t* parents, void* ws, size_t 
   const mea::PagedCache p = cache_of(c);
   hipStream_t s = static_cast<hipStream_t>(stream);
   int* w = static_cast<int*>(ws);
+  if (mea::paged_fork_small(p)) {
+    MEA_TRY(timed(K_FORK, s, [&] { return mea::launch_paged_fork(p, parents, s); }));
+    return MEA_OK;
+  }
   MEA_TRY(timed(K_FORK_READ, s, [&] { return mea::launch_paged_fork_read(p, parents, w, s); }));
   MEA_TRY(timed(K_FORK_WRITE, s, [&] { return mea::launch_paged_fork_write(p, parents, w, s); }));
   return MEA_OK;

@@ -72,6 +72,8 @@ hipError_t launch_paged_append_rows(const AppendParams& p, hipStream_t s);
 hipError_t launch_paged_accept_plan(const AcceptParams& p, hipStream_t s);
 hipError_t launch_paged_accept_rows(const AcceptParams& p, hipStream_t s);
 hipError_t launch_paged_truncate(const PagedCache& c, const int* lengths, hipStream_t s);
+bool paged_fork_small(const PagedCache& c);  // launch_paged_fork takes it; else the two launches
+hipError_t launch_paged_fork(const PagedCache& c, const int* parents, hipStream_t s);
 hipError_t launch_paged_fork_read(const PagedCache& c, const int* parents, int* ws, hipStream_t s);
 hipError_t launch_paged_fork_write(const PagedCache& c, const int* parents, const int* ws, hipStream_t s);
 hipError_t launch_paged_compact_plan(const PagedCache& c, int* ws, hipStream_t s);

@@ -12,7 +12,7 @@ enum KernelId {
   K_ATTN_DECODE, K_DECODE_COMBINE, K_SKINNY_GEMM, K_TABLE_GRAD, K_TABLE_ROWS,
   K_GROUPED_FWD, K_GROUPED_DQ, K_GROUPED_DKDV, K_GROUPED_JOIN, K_TREE_ATTN, K_TREE_COMBINE,
   K_APPEND_PLAN, K_APPEND_ROWS, K_ACCEPT_PLAN, K_ACCEPT_ROWS, K_TRUNCATE,
-  K_FORK_READ, K_FORK_WRITE, K_COMPACT_PLAN, K_COMPACT_MOVE, K_COUNT
+  K_FORK, K_FORK_READ, K_FORK_WRITE, K_COMPACT_PLAN, K_COMPACT_MOVE, K_COUNT
 };
 }  // namespace kernel_ids
 

@@ -58,23 +58,26 @@ __device__ __forceinline__ size_t row_at(const PagedCache& c, int page, int head
   return ((((size_t)page * c.Hkv + head) << c.lg_page) + row) * c.N;
 }
 
+// Bit e: page at + e is free, for the four pages of a thread.
+__device__ __forceinline__ int free_four(const PagedCache& c, int at) {
+  int bits = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bits |= (int)(at + e < c.pages && c.refs[min(at + e, c.pages - 1)] <= 0) << e;
+  return bits;
+}
 // The lowest `need` free pages into list, in order; returns how many there are
-// (all threads, after a barrier).
-__device__ __forceinline__ int free_pages(const PagedCache& c, int need, int* list, int* lds) {
+// (all threads, after a barrier). first: free_four() of the thread's first four
+// pages, which the caller requests before it knows the need.
+__device__ __forceinline__ int free_pages(const PagedCache& c, int need, int first, int* list, int* lds) {
   int found = 0;
   for (int p0 = 0; p0 < c.pages && found < need; p0 += 4 * kPlan) {
-    const int at = p0 + 4 * threadIdx.x;
-    int free[4], n = 0;
+    const int at = p0 + 4 * threadIdx.x, free = p0 == 0 ? first : free_four(c, at);
+    int total, rank = found + block_scan(__popc(free), lds, &total);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      free[e] = at + e < c.pages && c.refs[at + e] <= 0;
-      n += free[e];
-    }
-    int total, rank = found + block_scan(n, lds, &total);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (free[e] && rank < need) list[rank] = at + e;
-      rank += free[e];
+      const bool is = (free >> e & 1) != 0;
+      if (is && rank < need) list[rank] = at + e;
+      rank += is;
     }
     found += total;
   }
@@ -82,14 +85,12 @@ __device__ __forceinline__ int free_pages(const PagedCache& c, int need, int* li
   return min(found, need);
 }
 
-// Workspaces (ints): per sequence [start | copied page | need | offset | tail],
-// then the list of free pages.
+// Workspaces (ints): per sequence [start | copied page | three notes], then the list
+// of free pages.
 struct AppendWs {
-  int *start, *copied, *need, *off, *list;
+  int *start, *copied, *notes, *list;
 };
-__host__ __device__ AppendWs append_ws(int* ws, int S) {
-  return AppendWs{ws, ws + S, ws + 2 * S, ws + 3 * S, ws + 4 * S};
-}
+__host__ __device__ AppendWs append_ws(int* ws, int S) { return AppendWs{ws, ws + S, ws + 2 * S, ws + 5 * S}; }
 __host__ __device__ inline int tree_pages(int page, int n) { return (n + page - 1) / page + 1; }
 struct AcceptWs {
   int *base, *count, *need, *off, *shared, *old, *list;  // old: (S, J) pages before the call
@@ -104,17 +105,34 @@ __device__ __forceinline__ int new_rows(const AppendParams& p, int s) {
   return min(max(p.cu[s + 1], a), p.total) - a;
 }
 
+// Up to kPlan sequences, what the plan knows of them stays in LDS from the first
+// half to the second (9.3 -> 5.4 us at 64 sequences).
+template <int FIELDS>
+struct PlanNotes {
+  int* at[FIELDS];
+  __device__ __forceinline__ PlanNotes(int* lds, int* ws, int seqs) {
+    const bool fits = seqs <= kPlan;
+#pragma unroll
+    for (int f = 0; f < FIELDS; ++f) at[f] = fits ? lds + f * kPlan : ws + (size_t)f * seqs;
+  }
+  __device__ __forceinline__ int& operator()(int f, int s) const { return at[f][s]; }
+};
+
 __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendParams p) {
-  __shared__ int lds[kPlan / 64];
+  __shared__ int lds[kPlan / 64], notes_lds[3 * kPlan];
   const PagedCache& c = p.c;
   const AppendWs w = append_ws(p.ws, c.seqs);
+  enum { OLD, NEED, OFF };  // rows before; pages needed (-1: no room for the rows); first of them
+  const PlanNotes<3> note(notes_lds, w.notes, c.seqs);
   const int tid = threadIdx.x;
+  const int first_free = free_four(c, 4 * tid);
   int total = 0;
   for (int s0 = 0; s0 < c.seqs; s0 += kPlan) {
     const int s = s0 + tid;
-    int need = 0, copied = -1;
+    int need = 0, copied = -1, old = 0;
     if (s < c.seqs) {
-      const int old = length_of(c, s), more = new_rows(p, s);
+      const int more = new_rows(p, s);
+      old = length_of(c, s);
       if (more > 0 && more <= (c.max_pages << c.lg_page) - old) {
         need = pages_of(c, old + more) - pages_of(c, old);
         if ((old & (c.page - 1)) != 0) {
@@ -133,34 +151,47 @@ __global__ __launch_bounds__(kPlan) void append_plan_kernel(AppendParams p) {
     total += sum;
     if (s < c.seqs) {
       w.copied[s] = copied;
-      w.need[s] = need;
-      w.off[s] = off;
+      note(OLD, s) = old;
+      note(NEED, s) = need;
+      note(OFF, s) = off;
     }
   }
-  const int found = free_pages(c, total, w.list, lds);
-  // One wave per sequence from here on.
+  const int found = free_pages(c, total, first_free, w.list, lds);
+  // Who is served is settled; now the sequences' own entries.
+  for (int s = tid; s < c.seqs; s += kPlan) {
+    const int need = note(NEED, s), old = note(OLD, s), copied = w.copied[s];
+    const bool ok = need >= 0 && (need == 0 || note(OFF, s) + need <= found);
+    w.start[s] = ok ? old : -1;
+    if (!ok) {
+      w.copied[s] = -1;
+      atomicOr(c.status, need < 0 ? kNoRows : kNoPages);
+      note(NEED, s) = 0;
+    } else {
+      const int more = new_rows(p, s);
+      if (copied >= 0) atomicSub(&c.refs[copied], 1);
+      if (more > 0) c.lengths[s] = old + more;
+      // The first entry that is set: the copied page's, or the one behind the last.
+      note(OLD, s) = pages_of(c, old) - (copied >= 0 ? 1 : 0);
+    }
+  }
+  __syncthreads();
+  // Pages: a wave per sequence where there are many, a thread where there are one or two.
   const int lane = tid & 63;
-  for (int s = tid >> 6; s < c.seqs; s += kPlan / 64) {
-    const int need = w.need[s], off = w.off[s], copied = w.copied[s];
-    const bool ok = need >= 0 && (need == 0 || off + need <= found);
-    const int old = length_of(c, s), more = ok ? new_rows(p, s) : 0;
-    const int first = pages_of(c, old) - (copied >= 0 ? 1 : 0);
-    if (ok)
-      for (int j = lane; j < need; j += 64) {
-        const int page = w.list[off + j];
-        c.table[(size_t)s * c.max_pages + first + j] = page;
+  if (total <= 4 * c.seqs) {
+    for (int s = tid; s < c.seqs; s += kPlan)
+      for (int j = 0; j < note(NEED, s); ++j) {
+        const int page = w.list[note(OFF, s) + j];
+        c.table[(size_t)s * c.max_pages + note(OLD, s) + j] = page;
         c.refs[page] = 1;
       }
-    if (lane == 0) {
-      w.start[s] = ok ? old : -1;
-      if (ok && copied >= 0) atomicSub(&c.refs[copied], 1);
-      if (!ok) {
-        w.copied[s] = -1;
-        atomicOr(c.status, need < 0 ? kNoRows : kNoPages);
-      }
-      if (more > 0) c.lengths[s] = old + more;
-    }
+    return;
   }
+  for (int s = tid >> 6; s < c.seqs; s += kPlan / 64)
+    for (int j = lane; j < note(NEED, s); j += 64) {
+      const int page = w.list[note(OFF, s) + j];
+      c.table[(size_t)s * c.max_pages + note(OLD, s) + j] = page;
+      c.refs[page] = 1;
+    }
 }
 
 // Workgroups [0, row_wgs): 16-byte chunks of the new rows, chunk fastest. The
@@ -223,6 +254,7 @@ __global__ __launch_bounds__(kPlan) void accept_plan_kernel(AcceptParams p) {
   const PagedCache& c = p.c;
   const int J = tree_pages(c.page, p.n), tid = threadIdx.x;  // J <= 17
   const AcceptWs w = accept_ws(p.ws, c.seqs, J);
+  const int first_free = free_four(c, 4 * tid);
   int total = 0;
   for (int s0 = 0; s0 < c.seqs; s0 += kPlan) {
     const int s = s0 + tid;
@@ -249,7 +281,7 @@ __global__ __launch_bounds__(kPlan) void accept_plan_kernel(AcceptParams p) {
     total += sum;
     if (s < c.seqs) w.off[s] = off;
   }
-  const int found = free_pages(c, total, w.list, lds);
+  const int found = free_pages(c, total, first_free, w.list, lds);
   const int lane = tid & 63;
   for (int s = tid >> 6; s < c.seqs; s += kPlan / 64) {
     const int need = w.need[s], off = w.off[s], base = w.base[s], count = w.count[s], shared = w.shared[s];
@@ -371,6 +403,34 @@ __global__ __launch_bounds__(256) void fork_write_kernel(PagedCache c, const int
   if (threadIdx.x == 0) c.lengths[s] = len;
 }
 
+// Both halves in one workgroup, where the table fits its LDS (two launches: 3.5 + 2.6
+// us at 64 sequences of 65 entries).
+constexpr int kForkEntries = 12288;
+__global__ __launch_bounds__(kPlan) void fork_small_kernel(PagedCache c, const int* parents) {
+  __shared__ int rows[kForkEntries], len_s[kPlan], from_s[kPlan], pages_s[kPlan];
+  const int tid = threadIdx.x, n = c.seqs * c.max_pages;
+  int len = 0;
+  if (tid < c.seqs) {
+    const int from = parents[tid];
+    from_s[tid] = (unsigned)from < (unsigned)c.seqs ? from : -1;
+    len_s[tid] = len = length_of(c, tid);
+    pages_s[tid] = pages_of(c, len);
+  }
+  for (int i = tid; i < n; i += kPlan) rows[i] = c.table[i];
+  __syncthreads();
+  for (int i = tid; i < n; i += kPlan) {
+    const int s = i / c.max_pages, j = i - s * c.max_pages, from = from_s[s];
+    if (from == s) continue;
+    const int was = j < pages_s[s] ? rows[i] : -1;
+    const int now = from >= 0 && j < pages_s[from] ? rows[from * c.max_pages + j] : -1;
+    if (was == now) continue;  // the same page stays: nothing to count
+    if (in_pool(c, now)) atomicAdd(&c.refs[now], 1);
+    if (in_pool(c, was)) atomicSub(&c.refs[was], 1);
+    c.table[i] = now;
+  }
+  if (tid < c.seqs && from_s[tid] != tid) c.lengths[tid] = from_s[tid] >= 0 ? len_s[from_s[tid]] : 0;
+}
+
 // Workspace: [count of moves][page -> new page][sources][targets].
 __global__ __launch_bounds__(kPlan) void compact_plan_kernel(PagedCache c, int* ws) {
   __shared__ int lds[kPlan / 64];
@@ -430,7 +490,7 @@ __global__ __launch_bounds__(256) void compact_move_kernel(PagedCache c, const i
 
 }  // namespace
 
-size_t append_ws_ints(int seqs, int pages) { return 4 * (size_t)seqs + pages; }
+size_t append_ws_ints(int seqs, int pages) { return 5 * (size_t)seqs + pages; }
 size_t accept_ws_ints(int seqs, int pages, int page, int n) {
   return (size_t)seqs * (5 + tree_pages(page, n)) + pages;
 }
@@ -458,6 +518,13 @@ hipError_t launch_paged_accept_rows(const AcceptParams& p, hipStream_t s) {
 }
 hipError_t launch_paged_truncate(const PagedCache& c, const int* lengths, hipStream_t s) {
   hipLaunchKernelGGL(truncate_kernel, dim3(c.seqs), dim3(64), 0, s, c, lengths);
+  return hipGetLastError();
+}
+bool paged_fork_small(const PagedCache& c) {
+  return c.seqs <= kPlan && (int64_t)c.seqs * c.max_pages <= kForkEntries;
+}
+hipError_t launch_paged_fork(const PagedCache& c, const int* parents, hipStream_t s) {
+  hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kPlan), 0, s, c, parents);
   return hipGetLastError();
 }
 hipError_t launch_paged_fork_read(const PagedCache& c, const int* parents, int* ws, hipStream_t s) {
