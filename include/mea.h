@@ -101,7 +101,7 @@ enum {
   MEA_ERR_PAGE = -13,       /* page size is not 16, 32, 64, 128 or 256 */
   MEA_ERR_DTYPE = -14,      /* element type not supported */
   MEA_ERR_STRIDE = -15,     /* a stride is no multiple of 8 elements, or too large */
-  MEA_ERR_SCALE = -16       /* softmax scale not finite and positive */
+  MEA_ERR_SCALE = -16       /* softmax scale not in [2^-100, 2^100] */
 };
 
 /* Size of the static scratch buffer of mea_decode_static (per GPU). */
@@ -373,7 +373,7 @@ typedef struct mea_grouped {
   int64_t Hkv;    /* key/value heads */
   int64_t N;      /* head width: 32, 64, 128 or 256 */
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head; /* strides */
-  float scale;    /* > 0 */
+  float scale;    /* in [2^-100, 2^100] */
   int32_t dtype;  /* MEA_BF16 or MEA_FP16; the backward takes MEA_BF16 */
 } mea_grouped;
 

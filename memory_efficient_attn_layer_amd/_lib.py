@@ -210,9 +210,11 @@ def stream_of(device: torch.device) -> int:
 
 
 @functools.lru_cache(maxsize=512)
-def grouped_desc(*values) -> MeaGrouped:
-    """A mea_grouped of these values (the library only reads it)."""
-    return MeaGrouped(*values)
+def grouped_plan(*values) -> tuple[MeaGrouped, int]:
+    """A mea_grouped of these values (the library only reads it) and the workspace
+    bytes of its backward, kept by their values like ``plan``."""
+    d = MeaGrouped(*values)
+    return d, load().mea_grouped_workspace_bytes(d)
 
 
 @functools.lru_cache(maxsize=512)

@@ -950,7 +950,7 @@ const char* mea_strerror(int code) {
     case MEA_ERR_PAGE: return "pages must hold 16, 32, 64, 128 or 256 rows";
     case MEA_ERR_DTYPE: return "the element type must be bf16 or fp16 (backward: bf16)";
     case MEA_ERR_STRIDE: return "strides must be multiples of 8 elements, a row's at most 2^24";
-    case MEA_ERR_SCALE: return "the softmax scale must be finite and positive";
+    case MEA_ERR_SCALE: return "the softmax scale must lie in [2^-100, 2^100]";
     default: return "unknown status";
   }
 }

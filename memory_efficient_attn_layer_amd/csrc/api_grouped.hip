@@ -40,7 +40,8 @@ int check4(std::initializer_list<const void*> ps) {
 
 bool width_ok(int64_t N) { return N == 32 || N == 64 || N == 128 || N == 256; }
 bool dtype_ok(int32_t t) { return t == MEA_BF16 || t == MEA_FP16; }
-bool scale_ok(float s) { return s > 0.f && isfinite(s); }
+// (The kernels take log2(e) times it, and its inverse.)
+bool scale_ok(float s) { return s >= 0x1p-100f && s <= 0x1p100f; }
 // A row stride: a tile's rows are addressed with 32-bit byte offsets.
 bool row_stride_ok(int64_t s) { return s % 8 == 0 && s >= 0 && s <= (INT64_C(1) << 24); }
 bool stride_ok(int64_t s) { return s % 8 == 0 && s >= 0; }
@@ -333,7 +334,7 @@ int mea_tree_attn(const mea_paged* c, int64_t n, int64_t Hq, float scale, const 
   p.Hq = (int)Hq;
   const mea::TreeGrid g = tree_grid_of(c, n, Hq);
   p.want = g.want;
-  p.turn = g.turn;
+  p.full = g.full;
   p.row_groups = g.row_groups;
   p.sl2e = scale * 1.4426950408889634f;
   p.o = static_cast<bits16*>(o);

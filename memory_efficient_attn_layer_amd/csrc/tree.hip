@@ -63,50 +63,68 @@ __device__ __forceinline__ int wave_add(int v) {
   return v;
 }
 
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(v, off, 64);
+    if (lane >= off) v += y;
+  }
+  return v;
+}
+
+constexpr int kManySeqs = 4096;  // beyond, every sequence has the same number of items
+
 // The chunk size, and the sequence and chunk that are item `item` of a head.
 struct Chunk {
   int size, seq, chunk, count;  // seq < 0: no such item; count: the sequence's chunks (0 where it has no row)
 };
-// want: chunks of a head that run at one time; turn: granule of the size.
-__device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int turn, int item) {
+// want: chunks of a head that run at one time; turn: granule of the size; full:
+// the largest chunks of a sequence that is as long as the cache allows.
+__device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int turn, int full, int item) {
   const int lane = threadIdx.x & 63;
   auto len = [&](int s) { return min(max(c.lengths[s], 0), c.max_pages << c.lg_page); };
-  // Up to 64 sequences stay in a register.
-  const int len0 = lane < c.seqs ? len(lane) : 0;
+  Chunk r;
+  if (c.seqs > kManySeqs) {
+    r.size = kMaxChunk;
+    r.seq = item / full;
+    r.chunk = item - r.seq * full;
+    r.count = r.seq < c.seqs ? (len(r.seq) + kMaxChunk - 1) / kMaxChunk : 0;
+    if (r.seq >= c.seqs || r.chunk >= max(r.count, 1)) r.seq = -1;
+    return r;
+  }
+  // Lane l holds sequences l * per .. l * per + per - 1; the first in a register.
+  const int per = (c.seqs + 63) >> 6, mine0 = lane * per, len0 = mine0 < c.seqs ? len(mine0) : 0;
   auto sum = [&](auto f) {
-    int v = lane < c.seqs ? f(len0) : 0;
-    for (int s = 64 + lane; s < c.seqs; s += 64) v += f(len(s));
-    return wave_add(v);
+    int v = mine0 < c.seqs ? f(len0) : 0;
+    for (int s = mine0 + 1; s < min(mine0 + per, c.seqs); ++s) v += f(len(s));
+    return v;
   };
   auto whole = [&](int keys) { return (keys + turn - 1) / turn * turn; };
-  Chunk r;
-  // Sums of keys in units of 16, so that they fit 32 bits.
-  const int total = sum([](int n) { return (n + 15) >> 4; });
-  r.size = min(max(whole(((total + want - 1) / want) << 4), 2 * turn), kMaxChunk);
-  while (r.size < kMaxChunk && sum([&](int n) { return max((n + r.size - 1) / r.size, 1); }) > max(want, c.seqs))
-    r.size = min(whole(r.size + r.size / 16), kMaxChunk);
+  auto chunks = [&](int n) { return max((n + r.size - 1) / r.size, 1); };
+  // Few sequences: as many chunks as run at one time. Many: four times as many, which
+  // even out the rounds. (Sums of keys in units of 16, so that they fit 32 bits.)
+  const bool few = 2 * c.seqs <= want;
+  const int total = wave_add(sum([](int n) { return (n + 15) >> 4; })), parts = few ? want : 4 * want;
+  r.size = min(max(whole(((total + parts - 1) / parts) << 4), 2 * turn), kMaxChunk);
+  while (few && r.size < kMaxChunk && wave_add(sum(chunks)) > want) r.size = min(whole(r.size + r.size / 16), kMaxChunk);
   // Item -> (sequence, chunk): every sequence has one item at least.
-  int before = 0;
+  const int own = sum(chunks), up = wave_scan(own);
+  const unsigned long long at = __ballot(up > item);
   r.seq = -1;
-  for (int s0 = 0; s0 < c.seqs; s0 += 64) {
-    const int s = s0 + lane, n = s < c.seqs ? (s0 == 0 ? len0 : len(s)) : 0;
-    const int mine = s < c.seqs ? max((n + r.size - 1) / r.size, 1) : 0;
-    int up = mine;  // inclusive
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int y = __shfl_up(up, off, 64);
-      if (lane >= off) up += y;
-    }
-    const unsigned long long at = __ballot(before + up > item);
-    if (at != 0) {
-      const int l = __ffsll(at) - 1;
-      r.seq = __builtin_amdgcn_readfirstlane(s0 + l);
-      r.chunk = __builtin_amdgcn_readfirstlane(item - before - __shfl(up - mine, l, 64));
-      r.count = __builtin_amdgcn_readfirstlane((__shfl(n, l, 64) + r.size - 1) / r.size);
-      return r;
-    }
-    before += __shfl(up, 63, 64);
+  if (at == 0) return r;
+  const int l = __ffsll(at) - 1;
+  int rest = item - __shfl(up - own, l, 64), s = l;
+  if (per > 1) {
+    s = l * per + lane;
+    const int n = lane < per && s < c.seqs ? chunks(len(s)) : 0, to = wave_scan(n);
+    const int k = __ffsll(__ballot(to > rest)) - 1;
+    rest -= __shfl(to - n, k, 64);
+    s = l * per + k;
   }
+  r.seq = __builtin_amdgcn_readfirstlane(s);
+  r.chunk = __builtin_amdgcn_readfirstlane(rest);
+  r.count = __builtin_amdgcn_readfirstlane((len(r.seq) + r.size - 1) / r.size);
   return r;
 }
 
@@ -128,7 +146,7 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
   const int G = p.Hq / cc.Hkv, R = p.n * G;
   // Key heads fastest, then the row groups that read the same rows, then chunks.
   const int kv = blockIdx.x % cc.Hkv, grp = blockIdx.x / cc.Hkv, item = grp / p.row_groups;
-  const Chunk ck = find_chunk(cc, p.want, T::TURN, item);
+  const Chunk ck = find_chunk(cc, p.want, T::TURN, p.full, item);
   if (ck.seq < 0) return;
   const int s = ck.seq;
   const int len = __builtin_amdgcn_readfirstlane(min(max(cc.lengths[s], 0), cc.max_pages << cc.lg_page));
@@ -542,13 +560,15 @@ TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
   g.turn = N == 32 ? turn_of<32>(g.blocks) : N == 64 ? turn_of<64>(g.blocks) : N == 128 ? turn_of<128>(g.blocks) : turn_of<256>(g.blocks);
   const int64_t lanes = (int64_t)Hkv * g.row_groups;
   g.want = (int)(kSlots / lanes > 1 ? kSlots / lanes : 1);
-  // At most `want` chunks (or one per sequence) unless the largest chunk is too
-  // small; no more than the capacity has of the smallest.
-  const int64_t full = (int64_t)seqs * ((capacity + kMaxChunk - 1) / kMaxChunk);
+  // Few sequences: at most `want` chunks, many: 4 * want and one for each; or the
+  // largest chunks, if they are more; no more than the capacity has of the smallest.
+  g.full = (capacity + kMaxChunk - 1) / kMaxChunk;
   const int64_t most = (int64_t)seqs * ((capacity + 2 * g.turn - 1) / (2 * g.turn));
-  g.items = g.want > seqs ? g.want : seqs;
+  const int64_t full = (int64_t)seqs * g.full;
+  g.items = 2 * seqs <= g.want ? g.want : 4 * g.want + seqs;
   if (g.items < full) g.items = full;
-  if (g.items > most) g.items = most;
+  if (g.items > most && seqs <= kManySeqs) g.items = most;
+  if (seqs > kManySeqs) g.items = full;
   g.split = capacity > 2 * g.turn;
   return g;
 }

@@ -23,8 +23,8 @@ MAX_TOKEN_STRIDE = 1 << 24  # elements
 
 def _check_scale(scale, N: int) -> float:
     scale = 1.0 / math.sqrt(N) if scale is None else float(scale)
-    if not (0.0 < scale < float("inf")):
-        raise ValueError(f"scale={scale} must be finite and positive")
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        raise ValueError(f"scale={scale} must be in [2^-100, 2^100]")
     return scale
 
 
@@ -73,17 +73,18 @@ def _validate(q, k, v) -> None:
         raise RuntimeError("grouped_attn_varlen runs only on a ROCm GPU device (there is no CPU path)")
 
 
-def _desc(q, k, v, nseq: int, scale: float) -> _lib.MeaGrouped:
+def _plan(q, k, v, nseq: int, scale: float) -> tuple[_lib.MeaGrouped, int]:
+    """The call's descriptor and the workspace bytes of its backward."""
     total, Hq, N = q.shape
     sq, sk, sv = q.stride(), k.stride(), v.stride()
-    return _lib.grouped_desc(total, nseq, Hq, k.shape[1], N, sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], scale,
+    return _lib.grouped_plan(total, nseq, Hq, k.shape[1], N, sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], scale,
                              _lib.MEA_DTYPES[q.dtype])
 
 
 def _forward(q, k, v, cu_seqlens, scale, save):
     """(o, o_rest, lse), the last two None without ``save``; q, k, v as _tokens leaves them."""
     dev = q.device
-    d = _desc(q, k, v, cu_seqlens.shape[0] - 1, scale)
+    d, _ = _plan(q, k, v, cu_seqlens.shape[0] - 1, scale)
     total, Hq, N = q.shape
     o = torch.empty((total, Hq, N), device=dev, dtype=q.dtype)
     rest = torch.empty_like(o) if save else None
@@ -110,21 +111,21 @@ class GroupedAttentionFunction(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
+        if torch.is_grad_enabled():  # create_graph
+            raise RuntimeError("grouped_attn_varlen has no second derivative")
         q, k, v, cu, o, rest, lse = ctx.saved_tensors
-        lib = _lib.load()
         dev = q.device
-        dout = _aligned(grad_output.to(q.dtype))
-        d = _desc(q, k, v, cu.numel() - 1, ctx.scale)
+        dout = _aligned(grad_output)
+        d, ws_bytes = _plan(q, k, v, cu.shape[0] - 1, ctx.scale)
         dq, dk, dv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
-        ws_bytes = lib.mea_grouped_workspace_bytes(d)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
         with _lib.on_device(dev):
-            rc = lib.mea_grouped_bwd(d, cu.data_ptr(), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                     o.data_ptr(), rest.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                     ws.data_ptr(), ws_bytes, _lib.stream_of(dev))
-        _lib.check(rc, "mea_grouped_bwd")
+            rc = _lib.load().mea_grouped_bwd(d, cu.data_ptr(), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                             o.data_ptr(), rest.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                             dv.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_of(dev))
+        if rc != 0:
+            _lib.check(rc, "mea_grouped_bwd")
         return dq, dk, dv, None, None
 
 

@@ -121,7 +121,8 @@ class PagedKVCache:
         are taken as needed, the lowest free ones first, sequence by sequence; a
         page that other sequences hold too is copied before rows are written
         into it. A sequence for which there are too few pages, or that would
-        pass the capacity, stays as it is; see ``verify``."""
+        pass the capacity, stays as it is; see ``verify``. k and v must not be
+        parts of the pool."""
         self._on_gpu()
         S, (_, H, _, N) = self.sequences, self.k.shape
         packed = cu_seqlens is not None
@@ -156,7 +157,10 @@ class PagedKVCache:
         if not 1 <= n <= MAX_TREE:
             raise ValueError(f"n={n} must be in [1, {MAX_TREE}]")
         if not isinstance(path, torch.Tensor):
-            path = torch.tensor(path, dtype=torch.int32, device=self.k.device)
+            path = torch.tensor(path)
+            if path.dtype != torch.int64 or int(path.abs().max()) >= 1 << 31:
+                raise ValueError("path must hold 32-bit ints")
+            path = path.to(device=self.k.device, dtype=torch.int32)
         if (path.dim() != 2 or path.shape[0] != self.sequences or not 1 <= path.shape[1] <= n
                 or path.dtype != torch.int32 or path.device != self.k.device):
             raise ValueError(f"path must be an int32 tensor ({self.sequences}, 1 .. {n}) on {self.k.device}")
@@ -227,8 +231,10 @@ class PagedKVCache:
         dev = self.k.device
         if not isinstance(values, torch.Tensor) or (offsets is not None and values.device.type == "cpu"):
             values = torch.as_tensor(values)
-            if values.dim() != 1 or values.numel() != n:
-                raise ValueError(f"{name} must have {n} entries")
+            if values.dim() != 1 or values.numel() != n or values.dtype.is_floating_point or values.dtype == torch.bool:
+                raise ValueError(f"{name} must have {n} entries, all ints")
+            if int(values.min()) < -(1 << 31) or int(values.max()) >= 1 << 31:
+                raise ValueError(f"{name} must hold 32-bit ints")
             if offsets is not None:
                 from .attention import check_offsets
 

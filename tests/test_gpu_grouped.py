@@ -59,8 +59,23 @@ def test_forward_fp16(Hq, Hkv, lens, N):
     _check(LENS[lens], *_inputs(LENS[lens], Hq, Hkv, N, fp16, seed=N), backward=False)
 
 
-def test_more_sequences_than_lanes():
-    _check(LENS["many"], *_inputs(LENS["many"], 4, 2, 64, bf16))
+@pytest.mark.parametrize("nseq", [61, 62, 63, 64, 150])
+def test_as_many_sequences_as_lanes_and_more(nseq):
+    lens = LENS["many"][:nseq]
+    _check(lens, *_inputs(lens, 4, 2, 64, bf16))
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv,N", [([2500], 4, 1, 128), ([4100, 60], 2, 1, 64), ([1500, 1400], 8, 1, 256), ([700], 8, 1, 32)])
+def test_key_blocks_in_parts(lens, Hq, Hkv, N):
+    """Few key blocks with many query tiles: the gradients' sums are joined from parts."""
+    _check(lens, *_inputs(lens, Hq, Hkv, N, bf16, behind=70))
+
+
+def test_no_second_derivative():
+    leaves = [t.requires_grad_(True) for t in _inputs([20], 2, 1, 32, bf16)[:3]]
+    o = grouped_attn_varlen(*leaves, [0, 20])
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(o.float().square().sum(), leaves[0], create_graph=True)
 
 
 def test_tokens_of_no_sequence_get_zeros():

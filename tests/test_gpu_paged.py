@@ -208,6 +208,25 @@ def test_any_order_of_calls(S, H, N, page, pages, max_pages, dtype, seed):
         m.same(c)
 
 
+def test_large_tables():
+    """More sequences than a plan has threads, a table that is forked in two launches."""
+    S, H, N, page = 1100, 1, 32, 16
+    c = _cache(S, H, N, 2600, page, 12)
+    m = Model(c)
+    for it, n in enumerate((9, 10, 1)):
+        k, v = _rows(S * n, H, N, torch.bfloat16, it)
+        c.append(k.view(S, n, H, N).cuda(), v.view(S, n, H, N).cuda()), m.append(k, v, [n] * S)
+        m.same(c)
+        parents = [(s * 31 + it) % S if s % 3 else s for s in range(S)]
+        c.fork(parents), m.fork(parents)
+        m.same(c)
+        path, counts = [[2, 0]] * S, [s % 3 for s in range(S)]
+        c.accept(4, path, counts), m.accept(4, path, counts)
+        m.same(c)
+    c.compact(), m.compact()
+    m.same(c)
+
+
 def test_shared_pages_are_copied_by_every_writer():
     """Three sequences on one prompt; two of them write, one into the middle of the
     tree of the others."""
@@ -276,7 +295,8 @@ def test_refusals_on_the_gpu():
         c.accept(2, [[0, 1, 2]] * 2, [1, 1])
     with pytest.raises(ValueError):
         c.accept(2, [[0]], [1, 1])
-    for call in (lambda: c.truncate([1]), lambda: c.fork(torch.zeros(2, device="cuda")), lambda: c.free([2]),
+    for call in (lambda: c.truncate([0, 1 << 40]), lambda: c.truncate([0.0, 1.0]), lambda: c.accept(2, [[0.5], [1]], [1, 1]),
+                 lambda: c.truncate([1]), lambda: c.fork(torch.zeros(2, device="cuda")), lambda: c.free([2]),
                  lambda: c.accept(2, [[0], [1]], [1])):
         with pytest.raises(ValueError):
             call()

@@ -77,11 +77,19 @@ def test_long_contexts_are_split(Hq, Hkv, n, page, L):
     _check(c, Hq, n, _tree(3, n, 0) if n > 1 else None)
 
 
+@pytest.mark.parametrize("S,H,most", [(40, 8, 2500), (65, 1, 3000), (300, 1, 700), (700, 2, 100), (4097, 1, 40)])
+def test_many_sequences(S, H, most):
+    """More sequences than run at one time, than a wave has lanes, than are counted."""
+    lens = [(s * 7919) % most for s in range(S)]
+    lens[S // 2] = 9000 if S in (65, 4097) else most
+    c = _cache(lens, H, 32, 16, bf16)
+    _check(c, H, 1, None)
+
+
 @pytest.mark.parametrize("n,Hq", [(5, 4), (40, 4), (70, 4)])
 @pytest.mark.parametrize("lens", [[0, 0, 200], [2000, 3, 90]], ids=["short", "split"])
 def test_tokens_that_see_nothing_get_zeros(lens, n, Hq):
     """Masks without an entry: over no rows in front, nothing is left."""
-    lens = [min(lens[0], n) if lens[0] < n else lens[0], lens[1], lens[2]]
     c = _cache(lens, 2, 64, 16, bf16, room=n)
     mask = _tree(3, n, 3)
     mask[:, 2] = False
