@@ -146,8 +146,8 @@ struct TileLoad {
 // block on; S^T = K Q^T and O^T += V^T P^T, the query on the lane.
 //
 // Softmax: the running maximum is not followed score by score. A step first
-// takes the weights against the maximum m that is in force, and only where one
-// passes E::kMaxWeight (or is no number: the first step, m = -inf) finds the
+// takes the weights against the maximum m that is in force, and only where their
+// sum passes E::kMaxWeight (or is no number: the first step, m = -inf) finds the
 // step's own maximum, rescales and takes them again. The quotient is the same;
 // bf16 weights and fp32 sums have the range for it, and the exchange with the
 // other half of the wave leaves every other step.
@@ -236,17 +236,20 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_f
       }
       return s;
     };
-    float top_w;
+    u32x4 pf[2];
+    float ls;  // sum of the step's weights
     auto weigh = [&](f32x16& s) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i], p.sl2e, -m_i));
-      top_w = s[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top_w = fmaxf(top_w, s[i]);
+      for (int kst = 0; kst < 2; ++kst)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[kst][e] = E::pack(s[8 * kst + 2 * e], s[8 * kst + 2 * e + 1]);
+      ls = E::add_weights(0.f, s, pf);
     };
     f32x16 w = scores();
     weigh(w);
-    const bool over = !(top_w <= E::kMaxWeight);
+    const bool over = !(ls <= E::kMaxWeight);
     if (__any(over)) {
       const bool up = ((int)over | __shfl_xor((int)over, 32, 64)) != 0;  // (every lane takes part in the exchange)
       w = scores();  // (again: kept, they would cost every step sixteen registers)
@@ -267,12 +270,7 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 128 ? 2 : 1) void grouped_f
 #pragma unroll
       for (int i = 0; i < 16; ++i) l_exact += w[i];
     }
-    u32x4 pf[2];
-#pragma unroll
-    for (int kst = 0; kst < 2; ++kst)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pf[kst][e] = E::pack(w[8 * kst + 2 * e], w[8 * kst + 2 * e + 1]);
-    l_i = E::add_weights(l_i, w, pf);
+    l_i += ls;
     auto vread = [&](int kst, int db) -> u32x4 {
       const bits16* vr = vt + 16 * kst * N;
       return __builtin_shufflevector(lds_read_tr4(vr + voff[0][db]), lds_read_tr4(vr + voff[1][db]), 0, 1, 2, 3);
