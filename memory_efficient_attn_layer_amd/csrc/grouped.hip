@@ -819,10 +819,10 @@ unsigned query_grid(const GroupedParams& p) {
 }  // namespace
 
 // Parts of a key block's query tiles, at most eight: as many as fill the card, with
-// four tiles each at least; or as many as give its slots four workgroups each, which
+// four tiles each at least; or as many as give its slots three workgroups each, which
 // evens out the causal blocks' lengths, where a part has 64 tiles at least, whose
 // time makes up for the sums' way through memory. (T = 8192 x 2, 16 / 4 heads of 128,
-// 1 / 4 parts: dK/dV with the join 1394 / 864 us; 24 sequences of 1100 on average, 8 /
+// dK/dV with the join: 1 part 1394 us, 2, 3, 4 parts 948, 921, 910; 24 sequences of 1100 on average, 8 /
 // 4 heads of 64, 17 tiles a block: 147 / 199 us.)
 int dkdv_parts(int total, int nseq, int Hq, int Hkv, int N) {
   const int64_t slots = 256 * (N <= 64 ? 3 : N == 128 ? 2 : 1), blocks = (int64_t)(total / 128 + nseq) * Hkv;

@@ -14,7 +14,7 @@
 // is the group's own. A wave alone in its group (RW = 1) waits for its own loads
 // only, no barrier in the loop, and the other waves' loads stay in flight meanwhile;
 // sharing waves pass one barrier per tile. Two workgroups a CU, two waves a SIMD where
-// their registers allow it: a wave alone runs its products and exponentials one
+// their registers allow it, or one of twice the waves: a wave alone runs its products and exponentials one
 // after the other.
 //
 // Chunks: the host knows capacities, not lengths. Every workgroup reads all
@@ -37,17 +37,22 @@ namespace {
 
 constexpr int kMaxChunk = 8192;             // keys
 constexpr int kTab = kMaxChunk / 16 + 2;    // its table entries at 16 rows a page
-constexpr int kSlots = 512;                 // workgroups at one time: two per CU
 
-// RW waves share a tile, KG groups of them run; rings of NS tiles that fill 64 KB.
+// RW waves share a tile, KG groups of them run; rings of NS tiles, 64 KB and two
+// workgroups a CU. Four waves a tile: tiles and rings of twice the size and one
+// workgroup a CU, whose two groups join their sums in LDS, so that half as many go
+// through memory. (N = 128, 16 sequences of up to 4096 rows, 32 tokens: 41.0 us with two
+// workgroups of one group, 38.6 so, 37.4 with four tiles of half the size; one of
+// 131072 rows, 64 tokens: 133.2, 132.0, 135.4.)
 template <int N, int RW>
 struct Tile {
-  static constexpr int ST = N >= 128 ? 1 : 128 / N;  // 32-key steps
+  static constexpr int ST = (N >= 128 ? 1 : 128 / N) * (RW == 4 && N < 256 ? 2 : 1);  // 32-key steps
   static constexpr int KEYS = 32 * ST, ELEMS = KEYS * N;
-  static constexpr int KG = RW == 4 || N == 256 ? 1 : 2, NS = (N == 256 ? 2 : 4) / KG;
+  static constexpr int KG = N == 256 ? 1 : 2, NS = 2;
   static constexpr int WAVES = RW * KG, LOADS = ELEMS / 8 / 64 / RW;
   static constexpr int RING = NS * 2 * ELEMS;  // [stage][K | V]
   static constexpr int TURN = KEYS * KG;  // keys of one turn of the workgroup
+  static constexpr int SLOTS = RW == 4 ? 256 : 512;  // workgroups at one time
 };
 
 // s_waitcnt vmcnt(n), and nothing that reads or writes memory moves across it.
@@ -282,16 +287,19 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
         return w;
       };
       f32x16 w = scores();
-      float top_w;
+      u32x4 pf[2];
+      float ls;  // sum of the step's weights
       auto weigh = [&](float m) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i] = fast_exp2(__builtin_fmaf(w[i], p.sl2e, -m));
-        top_w = w[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top_w = fmaxf(top_w, w[i]);
+        for (int kst = 0; kst < 2; ++kst)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pf[kst][e] = E::pack(w[8 * kst + 2 * e], w[8 * kst + 2 * e + 1]);
+        ls = E::add_weights(0.f, w, pf);
       };
       weigh(m_i);
-      const bool over = !(top_w <= E::kMaxWeight);
+      const bool over = !(ls <= E::kMaxWeight);
       if (__any(over)) {
         const bool up = ((int)over | __shfl_xor((int)over, 32, 64)) != 0;  // (every lane takes part in the exchange)
         w = scores();
@@ -308,12 +316,7 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
         // No key seen: weights exp2(-inf - 0) = 0. (NaN scores stay NaN.)
         weigh(mn == -INFINITY ? 0.f : mn);
       }
-      u32x4 pf[2];
-#pragma unroll
-      for (int kst = 0; kst < 2; ++kst)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pf[kst][e] = E::pack(w[8 * kst + 2 * e], w[8 * kst + 2 * e + 1]);
-      l_i = E::add_weights(l_i, w, pf);
+      l_i += ls;
       auto vread = [&](int kst, int db) -> u32x4 {
         const bits16* vr = vt + 16 * kst * N;
         return __builtin_shufflevector(lds_read_tr4(vr + voff[0][db]), lds_read_tr4(vr + voff[1][db]), 0, 1, 2, 3);
@@ -533,8 +536,8 @@ hipError_t launch_combine(const TreeParams& p, hipStream_t s) {
   const int rows = p.n * p.Hq;
   by_width(p.c.N, [&](auto n) {
     constexpr int N = decltype(n)::value, GR = 1024 / N;
-    // A workgroup a row while that leaves them few (1024 rows: 8.1 us so, 9.9 with a
-    // row for each 32 lanes; 8192 rows: 24.1 / 6.9 us, N = 128).
+    // A workgroup a row while that leaves them few (N = 128; 1024 rows of 64 chunks:
+    // 9.3 us so, 27 with a row for each 32 lanes; 8192 rows of 8 chunks: 24 / 11).
     if ((int64_t)p.c.seqs * rows <= 2048)
       hipLaunchKernelGGL((tree_combine_kernel<E, N, true>), dim3(p.c.seqs, rows), dim3(256), 0, s, p);
     else
@@ -546,6 +549,10 @@ hipError_t launch_combine(const TreeParams& p, hipStream_t s) {
 template <int N>
 int turn_of(int blocks) {
   return blocks == 1 ? Tile<N, 1>::TURN : blocks == 2 ? Tile<N, 2>::TURN : Tile<N, 4>::TURN;
+}
+template <int N>
+int slots_of(int blocks) {
+  return blocks == 1 ? Tile<N, 1>::SLOTS : blocks == 2 ? Tile<N, 2>::SLOTS : Tile<N, 4>::SLOTS;
 }
 
 }  // namespace
@@ -559,7 +566,8 @@ TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
   g.row_groups = (need + g.blocks - 1) / g.blocks;
   g.turn = N == 32 ? turn_of<32>(g.blocks) : N == 64 ? turn_of<64>(g.blocks) : N == 128 ? turn_of<128>(g.blocks) : turn_of<256>(g.blocks);
   const int64_t lanes = (int64_t)Hkv * g.row_groups;
-  g.want = (int)(kSlots / lanes > 1 ? kSlots / lanes : 1);
+  const int slots = N == 32 ? slots_of<32>(g.blocks) : N == 64 ? slots_of<64>(g.blocks) : N == 128 ? slots_of<128>(g.blocks) : slots_of<256>(g.blocks);
+  g.want = (int)(slots / lanes > 1 ? slots / lanes : 1);
   // Few sequences: at most `want` chunks, many: 4 * want and one for each; or the
   // largest chunks, if they are more; no more than the capacity has of the smallest.
   g.full = (capacity + kMaxChunk - 1) / kMaxChunk;
