@@ -822,8 +822,8 @@ unsigned query_grid(const GroupedParams& p) {
 // four tiles each at least; or as many as give its slots three workgroups each, which
 // evens out the causal blocks' lengths, where a part has 64 tiles at least, whose
 // time makes up for the sums' way through memory. (T = 8192 x 2, 16 / 4 heads of 128,
-// dK/dV with the join: 1 part 1394 us, 2, 3, 4 parts 948, 921, 910; 24 sequences of 1100 on average, 8 /
-// 4 heads of 64, 17 tiles a block: 147 / 199 us.)
+// dK/dV with the join: 1 part 1394 us, 2, 3, 4 parts 948, 921, 910; 24 sequences of
+// 1100 on average, 8 / 4 heads of 64, 17 tiles a block: 1 part 147 us, 4 parts 199.)
 int dkdv_parts(int total, int nseq, int Hq, int Hkv, int N) {
   const int64_t slots = 256 * (N <= 64 ? 3 : N == 128 ? 2 : 1), blocks = (int64_t)(total / 128 + nseq) * Hkv;
   const int64_t tiles = (int64_t)(total / nseq) * (Hq / Hkv) / (2 * (N >= 128 ? 32 : 64));  // of a block, on average

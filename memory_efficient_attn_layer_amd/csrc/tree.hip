@@ -18,9 +18,9 @@
 // after the other.
 //
 // Chunks: the host knows capacities, not lengths. Every workgroup reads all
-// lengths and settles the chunk size by itself: the smallest, in whole turns of the
-// waves, that gives at most as many chunks as run at one time, so that they end
-// together. Several chunks of a sequence leave fp32 sums, which the second launch
+// lengths and settles the chunk size by itself: where sequences are few, the smallest,
+// in whole turns of the waves, that gives at most as many chunks as run at one time,
+// so that they end together. Several chunks of a sequence leave fp32 sums, which the second launch
 // adds in order.
 //
 // Pages: the chunk's table entries are read once into LDS; pages hold sixteen rows
@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kMaxChunk = 8192;             // keys
 constexpr int kTab = kMaxChunk / 16 + 2;    // its table entries at 16 rows a page
+constexpr int kSeenPitch = kMaxTree / 32 + 1;  // words of a mask's row (the last is not used)
 
 // RW waves share a tile, KG groups of them run; rings of NS tiles, 64 KB and two
 // workgroups a CU. Four waves a tile: tiles and rings of twice the size and one
@@ -62,22 +63,21 @@ __device__ __forceinline__ void wait_loads() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-__device__ __forceinline__ int wave_add(int v) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+// Inclusive sum over the wave's lanes, every lane taking part: within rows of sixteen
+// lanes by DPP row shifts, then the last lane of a row, and of half a wave, to those behind.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
   return v;
 }
+// (By a permute, not a scalar register: the loop's counts in scalars cost the kernel spills.)
+__device__ __forceinline__ int wave_add(int v) { return __shfl(wave_scan(v), 63, 64); }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(v, off, 64);
-    if (lane >= off) v += y;
-  }
-  return v;
-}
-
+constexpr int kLeast = 2048;      // keys of a chunk where sequences are many
 constexpr int kManySeqs = 4096;  // beyond, every sequence has the same number of items
 
 // The chunk size, and the sequence and chunk that are item `item` of a head.
@@ -108,10 +108,13 @@ __device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int t
   auto whole = [&](int keys) { return (keys + turn - 1) / turn * turn; };
   auto chunks = [&](int n) { return max((n + r.size - 1) / r.size, 1); };
   // Few sequences: as many chunks as run at one time. Many: four times as many, which
-  // even out the rounds. (Sums of keys in units of 16, so that they fit 32 bits.)
+  // even out the rounds, but none below kLeast keys, which a workgroup's start and the
+  // sums' way through memory would cost more than (64 sequences of up to 1024 rows of
+  // 8 heads, one token: chunks of 150 keys 61 us, whole sequences 48; of up to 2048:
+  // 90 and 82). (Sums of keys in units of 16, so that they fit 32 bits.)
   const bool few = 2 * c.seqs <= want;
   const int total = wave_add(sum([](int n) { return (n + 15) >> 4; })), parts = few ? want : 4 * want;
-  r.size = min(max(whole(((total + parts - 1) / parts) << 4), 2 * turn), kMaxChunk);
+  r.size = min(max(whole(((total + parts - 1) / parts) << 4), few ? 2 * turn : kLeast), kMaxChunk);
   while (few && r.size < kMaxChunk && wave_add(sum(chunks)) > want) r.size = min(whole(r.size + r.size / 16), kMaxChunk);
   // Item -> (sequence, chunk): every sequence has one item at least.
   const int own = sum(chunks), up = wave_scan(own);
@@ -141,6 +144,7 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
   static_assert(KG == 1 || KG * T::RING >= RW * DB * 16 * 64 * 2, "the exchange of one group's fp32 sums fits the rings");
   __shared__ __attribute__((aligned(16))) bits16 smem_all[KG * T::RING];
   __shared__ int tab[kTab];
+  __shared__ uint32_t seen_s[RW * 32 * kSeenPitch];
   __shared__ float xm[KG > 1 ? RW * 64 : 1], xl[KG > 1 ? RW * 64 : 1];
 
   const PagedCache& cc = p.c;
@@ -158,6 +162,7 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
   const int ctx = max(len - p.n, 0), lead = p.n - (len - ctx);  // lead: tokens in front of a short sequence's rows
   const int k_begin = ck.chunk * ck.size, k_end = min(k_begin + ck.size, len);
   const int r0 = ((grp - item * p.row_groups) * RW + rw) * 32;  // first query row of the wave
+  const int tok0 = (grp - item * p.row_groups) * RW * 32 / G;   // first token of the workgroup
 
   // Query row r = i * G + g: token i, head kv * G + g.
   const int r = min(r0 + c, R - 1), qi = r / G;
@@ -232,42 +237,34 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
 #pragma unroll
       for (int db = 0; db < DB; ++db) voff[x][db] = swz_off<CH>(tr_row + 8 * x, 32 * db + tr_col);
 
-    // Whether the token qi sees row `key`, for the sixteen keys that this lane has
-    // of a step (bit i: key kb0 + 8 (i >> 2) + 4 h + (i & 3)). No branch in it that
-    // depends on the lane: sixteen loads in flight together.
-    const unsigned char* mask = p.mask == nullptr ? nullptr : p.mask + s * p.mask_seq;
-    auto visible = [&](int kb0, int qi) -> uint32_t {
-      uint32_t bits = 0, in = 0;
-      if (mask == nullptr) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = kb0 + 8 * (i >> 2) + 4 * h + (i & 3);
-          bits |= (uint32_t)(key - ctx + lead <= qi) << i;
-        }
+    // Whether the token qi sees the sixteen rows that this lane has of a step (bit i:
+    // key kb0 + 8 (i >> 2) + 4 h + (i & 3)), from the 32 of the step, bit by bit.
+    auto visible = [&](int kb0) -> uint32_t {
+      const int at = kb0 - ctx + lead;  // token of the first row; below 0: rows that all see
+      uint32_t w;
+      if (p.mask == nullptr) {
+        const int d = qi - at + 1;  // rows that qi sees
+        w = d >= 32 ? ~0u : (1u << max(d, 0)) - 1u;
       } else {
-        const unsigned char* row = mask + (int64_t)qi * p.n;
-        uint32_t m[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int token = kb0 + 8 * (i >> 2) + 4 * h + (i & 3) - ctx + lead;
-          m[i] = row[min(max(token, 0), p.n - 1)];
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = kb0 + 8 * (i >> 2) + 4 * h + (i & 3);
-          bits |= (uint32_t)((m[i] != 0) | (key < ctx)) << i;
-        }
+        const uint32_t* row = seen_s + (qi - tok0) * kSeenPitch;
+        if (at >= 0)
+          w = (uint32_t)(((uint64_t)row[(at >> 5) + 1] << 32 | row[at >> 5]) >> (at & 31));
+        else
+          w = at <= -32 ? ~0u : (row[0] << -at | ((1u << -at) - 1u));
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) in |= (uint32_t)(kb0 + 8 * (i >> 2) + 4 * h + (i & 3) < k_end) << i;
+      const int rows = k_end - kb0;
+      if (rows < 32) w &= (1u << rows) - 1u;
+      w = w >> (4 * h) & 0x0F0F0F0Fu;
+      w = (w | w >> 4) & 0x00FF00FFu;
+      w = (w | w >> 8) & 0xFFFFu;
       if (!all_in) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = min(kb0 + 8 * (i >> 2) + 4 * h + (i & 3), k_end - 1);
-          in &= ~((uint32_t)(tab[(key >> cc.lg_page) - first] < 0) << i);
+          w &= ~((uint32_t)(tab[(key >> cc.lg_page) - first] < 0) << i);
         }
       }
-      return bits & in;
+      return w;
     };
 
     // One 32-key step, as in the forward of the packed prompts; MASK: some row may
@@ -275,7 +272,7 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
     bool hidden = false;  // a masked step's V held infinities or NaN, left out there
     auto step = [&](const bits16* kt, const bits16* vt, int kb0, auto mask_tag) {
       constexpr bool MASK = decltype(mask_tag)::value;
-      const uint32_t seen = MASK ? visible(kb0, qi) : 0;
+      const uint32_t seen = MASK ? visible(kb0) : 0;
       auto scores = [&] {
         f32x16 w = zero16();
 #pragma unroll
@@ -346,6 +343,25 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
     const bool idle = r0 >= R;  // no query rows left for this wave
 #pragma unroll
     for (int i = 0; i < NS - (RW > 1 ? 1 : 0); ++i) issue(kg + i * KG, i);
+    // The mask's rows of the workgroup's tokens, where the chunk has rows of the tree,
+    // as bits, while the first tiles are under way.
+    if (p.mask != nullptr && k_end > ctx) {
+      const unsigned char* mask = p.mask + s * p.mask_seq;
+      const int rows = min(((grp - item * p.row_groups) * RW * 32 + RW * 32 - 1) / G, p.n - 1) - tok0 + 1;
+      for (int j = lane; j - lane < p.n; j += 64)
+        for (int i = wave; i < rows; i += 4 * WAVES) {
+          unsigned char b[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) b[u] = mask[(int64_t)(tok0 + min(i + u * WAVES, rows - 1)) * p.n + min(j, p.n - 1)];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const unsigned long long bits = __ballot(b[u] != 0);
+            if (i + u * WAVES < rows && lane < 2)
+              seen_s[(i + u * WAVES) * kSeenPitch + (j - lane) / 32 + lane] = (uint32_t)(bits >> (32 * lane));
+          }
+        }
+      __syncthreads();
+    }
     // RW = 1: the tile's stage is filled again once it is read. RW > 1: after the
     // barrier that ends the wait for a tile, every wave has read the tile before it.
     const int turns = (nt + KG - 1) / KG;
@@ -380,7 +396,7 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
       for (int t = kg; t < nt; t += KG)
         for (int kb0 = k_begin + t * T::KEYS; kb0 < min(k_begin + (t + 1) * T::KEYS, k_end); kb0 += 32) {
           if (kb0 + 32 <= free_end) continue;
-          const uint32_t seen = visible(kb0, qi);
+          const uint32_t seen = visible(kb0);
           // Bits of the lane's own half; the other half's keys come from lane ^ 32.
           const uint32_t other = __shfl_xor(seen, 32, 64), lo = h == 0 ? seen : other, hi = h == 0 ? other : seen;
 #pragma unroll 1
@@ -571,13 +587,14 @@ TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
   // Few sequences: at most `want` chunks, many: 4 * want and one for each; or the
   // largest chunks, if they are more; no more than the capacity has of the smallest.
   g.full = (capacity + kMaxChunk - 1) / kMaxChunk;
-  const int64_t most = (int64_t)seqs * ((capacity + 2 * g.turn - 1) / (2 * g.turn));
+  const int least = 2 * seqs <= g.want ? 2 * g.turn : kLeast;
+  const int64_t most = (int64_t)seqs * ((capacity + least - 1) / least);
   const int64_t full = (int64_t)seqs * g.full;
   g.items = 2 * seqs <= g.want ? g.want : 4 * g.want + seqs;
   if (g.items < full) g.items = full;
   if (g.items > most && seqs <= kManySeqs) g.items = most;
   if (seqs > kManySeqs) g.items = full;
-  g.split = capacity > 2 * g.turn;
+  g.split = capacity > (seqs > kManySeqs ? kMaxChunk : least);
   return g;
 }
 
