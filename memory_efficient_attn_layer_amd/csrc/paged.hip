@@ -431,28 +431,36 @@ __global__ __launch_bounds__(kPlan) void fork_small_kernel(PagedCache c, const i
   if (tid < c.seqs && from_s[tid] != tid) c.lengths[tid] = from_s[tid] >= 0 ? len_s[from_s[tid]] : 0;
 }
 
-// Workspace: [count of moves][page -> new page][sources][targets].
+// Workspace: [count of moves][page -> new page][sources][targets]. Four pages a
+// thread and pass (one page: 11.3 us, four: 6.5, of 3100 pages).
 __global__ __launch_bounds__(kPlan) void compact_plan_kernel(PagedCache c, int* ws) {
   __shared__ int lds[kPlan / 64];
   int *map = ws + 1, *src = map + c.pages, *dst = src + c.pages;
+  const int first = free_four(c, 4 * threadIdx.x);
+  auto free_at = [&](int at) { return at < 4 * kPlan ? first : free_four(c, at); };
+  auto real = [&](int at) { return at >= c.pages ? 0 : at + 4 <= c.pages ? 15 : (1 << (c.pages - at)) - 1; };
   int live = 0;
-  for (int p0 = 0; p0 < c.pages; p0 += kPlan) {
+  for (int p0 = 0; p0 < c.pages; p0 += 4 * kPlan) {
     int total;
-    const int at = p0 + threadIdx.x;
-    block_scan(at < c.pages && c.refs[at] > 0, lds, &total);
+    const int at = p0 + 4 * threadIdx.x;
+    block_scan(__popc(real(at) & ~free_at(at)), lds, &total);
     live += total;
   }
   int n_src = 0, n_dst = 0;
-  for (int p0 = 0; p0 < c.pages; p0 += kPlan) {
-    const int at = p0 + threadIdx.x;
-    const bool used = at < c.pages && c.refs[at] > 0;
-    const bool moves = used && at >= live, hole = at < live && !used;
+  for (int p0 = 0; p0 < c.pages; p0 += 4 * kPlan) {
+    const int at = p0 + 4 * threadIdx.x, free = free_at(at), used = real(at) & ~free;
+    const int low = at >= live ? 0 : at + 4 <= live ? 15 : (1 << (live - at)) - 1;  // pages below live
+    const int moves = used & ~low, holes = free & low;
     int total;
-    // Holes lie before the moving pages, but both may share a chunk.
-    const int packed = block_scan((moves ? 1 : 0) | (hole ? 1 << 16 : 0), lds, &total);
-    if (moves) src[n_src + (packed & 0xFFFF)] = at;
-    if (hole) dst[n_dst + (packed >> 16)] = at;
-    if (at < c.pages) map[at] = at;
+    // Holes lie before the moving pages, but both may share a pass: a half each, 4 * kPlan at most.
+    const int packed = block_scan(__popc(moves) | __popc(holes) << 16, lds, &total);
+    int to_src = n_src + (packed & 0xFFFF), to_dst = n_dst + (packed >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if ((moves >> e & 1) != 0) src[to_src++] = at + e;
+      if ((holes >> e & 1) != 0) dst[to_dst++] = at + e;
+      if (at + e < c.pages) map[at + e] = at + e;
+    }
     n_src += total & 0xFFFF;
     n_dst += total >> 16;
   }

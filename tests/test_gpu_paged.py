@@ -227,6 +227,22 @@ def test_large_tables():
     m.same(c)
 
 
+@pytest.mark.parametrize("pages,held", [(4099, 1), (4096, 4096), (9001, 3000), (9001, 8200), (8193, 0)])
+def test_pools_of_many_pages_are_compacted(pages, held):
+    """More pages than one pass of the plan takes; none to move, none free, most of both."""
+    c = _cache(4, 1, 32, pages, 16, pages // 4 + 1)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(held))[:held].to(torch.int32)
+    for s in range(4):
+        mine = order[s::4]
+        c.table[s, : len(mine)] = mine.cuda()
+        c.lengths[s] = 16 * len(mine)
+    c.refs[order.long().cuda()] = 1
+    m = Model(c)
+    c.compact()
+    m.compact()
+    m.same(c)
+
+
 def test_shared_pages_are_copied_by_every_writer():
     """Three sequences on one prompt; two of them write, one into the middle of the
     tree of the others."""
