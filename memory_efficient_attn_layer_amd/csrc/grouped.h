@@ -95,8 +95,9 @@ struct TreeParams {
   float* part;
 };
 __host__ __device__ inline size_t tree_head_floats(int seqs) { return (2 * (size_t)seqs + 3) & ~(size_t)3; }
-// How a call is cut up. split: a sequence may have several chunks, whose sums the
-// second launch joins.
+// How a call is cut up. full: the largest chunks of a sequence of all the rows that it
+// can have; split: a sequence may have several chunks, whose sums the second launch
+// joins.
 struct TreeGrid {
   int blocks, row_groups, turn, want, full;
   int64_t items;

@@ -78,19 +78,20 @@ __device__ __forceinline__ int wave_scan(int v) {
 __device__ __forceinline__ int wave_add(int v) { return __shfl(wave_scan(v), 63, 64); }
 
 constexpr int kLeast = 2048;      // keys of a chunk where sequences are many
-constexpr int kManySeqs = 4096;  // beyond, every sequence has the same number of items
+// Beyond so many, or where their rows could be 2^35 (the count of them in 32 bits),
+// every sequence has the same number of items, of kMaxChunk keys.
+constexpr int kManySeqs = 4096;
 
 // The chunk size, and the sequence and chunk that are item `item` of a head.
 struct Chunk {
   int size, seq, chunk, count;  // seq < 0: no such item; count: the sequence's chunks (0 where it has no row)
 };
-// want: chunks of a head that run at one time; turn: granule of the size; full:
-// the largest chunks of a sequence that is as long as the cache allows.
+// want, full: of TreeGrid; turn: granule of the size.
 __device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int turn, int full, int item) {
   const int lane = threadIdx.x & 63;
   auto len = [&](int s) { return min(max(c.lengths[s], 0), c.max_pages << c.lg_page); };
   Chunk r;
-  if (c.seqs > kManySeqs) {
+  if (want == 0) {
     r.size = kMaxChunk;
     r.seq = item / full;
     r.chunk = item - r.seq * full;
@@ -574,7 +575,8 @@ int slots_of(int blocks) {
 }  // namespace
 
 // blocks: waves of 32 query rows that share a workgroup's tiles; want: chunks of a
-// head that run at one time; items: a bound of a head's chunks.
+// head that run at one time (0: chunks of the largest size); items: a bound of a
+// head's chunks.
 TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
   TreeGrid g;
   const int need = (rows + 31) / 32;
@@ -583,18 +585,24 @@ TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
   g.turn = N == 32 ? turn_of<32>(g.blocks) : N == 64 ? turn_of<64>(g.blocks) : N == 128 ? turn_of<128>(g.blocks) : turn_of<256>(g.blocks);
   const int64_t lanes = (int64_t)Hkv * g.row_groups;
   const int slots = N == 32 ? slots_of<32>(g.blocks) : N == 64 ? slots_of<64>(g.blocks) : N == 128 ? slots_of<128>(g.blocks) : slots_of<256>(g.blocks);
-  g.want = (int)(slots / lanes > 1 ? slots / lanes : 1);
+  g.full = (capacity + kMaxChunk - 1) / kMaxChunk;
+  const int64_t full = (int64_t)seqs * g.full;
+  if (seqs > kManySeqs || (int64_t)seqs * (capacity / 16 + 1) >= INT64_C(1) << 31) {
+    g.want = 0;
+    g.items = full;
+    g.split = capacity > kMaxChunk;
+    return g;
+  }
   // Few sequences: at most `want` chunks, many: 4 * want and one for each; or the
   // largest chunks, if they are more; no more than the capacity has of the smallest.
-  g.full = (capacity + kMaxChunk - 1) / kMaxChunk;
-  const int least = 2 * seqs <= g.want ? 2 * g.turn : kLeast;
+  g.want = (int)(slots / lanes > 1 ? slots / lanes : 1);
+  const bool few = 2 * seqs <= g.want;
+  const int least = few ? 2 * g.turn : kLeast;
   const int64_t most = (int64_t)seqs * ((capacity + least - 1) / least);
-  const int64_t full = (int64_t)seqs * g.full;
-  g.items = 2 * seqs <= g.want ? g.want : 4 * g.want + seqs;
+  g.items = few ? g.want : 4 * g.want + seqs;
   if (g.items < full) g.items = full;
-  if (g.items > most && seqs <= kManySeqs) g.items = most;
-  if (seqs > kManySeqs) g.items = full;
-  g.split = capacity > (seqs > kManySeqs ? kMaxChunk : least);
+  if (g.items > most) g.items = most;
+  g.split = capacity > least;
   return g;
 }
 

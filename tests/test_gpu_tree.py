@@ -86,6 +86,31 @@ def test_many_sequences(S, H, most):
     _check(c, H, 1, None)
 
 
+@pytest.mark.parametrize("one", [False, True], ids=["each", "shared"])
+@pytest.mark.parametrize("Hq,Hkv,N", [(1, 1, 128), (3, 1, 32), (10, 2, 64)])
+@pytest.mark.parametrize("n", [2, 31, 32, 33, 64, 65, 129, 200, 256])
+def test_any_mask(n, Hq, Hkv, N, one):
+    """Masks of no shape at all, tokens that see later ones among them, the new rows
+    at any place of a tile, of a page, of a chunk."""
+    lens = [n, n + 31, n + 97, n // 2, n + 1000, 1, n + 4096 - 13]
+    c = _cache(lens, Hkv, N, 32, bf16, seed=n)
+    g = torch.Generator("cuda").manual_seed(n)
+    shape = (n, n) if one else (len(lens), n, n)
+    _check(c, Hq, n, torch.rand(shape, device="cuda", generator=g) < 0.3)
+
+
+def test_capacities_whose_rows_pass_32_bits():
+    """Tables so long that the sequences could have 2^35 rows."""
+    S, M = 33, (1 << 22) - 1
+    lens = [9000] + [(7 * s) % 90 for s in range(1, S)]
+    small = _cache(lens, 1, 32, 256, bf16)
+    table = torch.full((S, M), -1, device="cuda", dtype=torch.int32)
+    table[:, : small.table.shape[1]] = small.table
+    c = PagedKVCache(small.k, small.v, table, small.lengths, small.refs, small.status)
+    q, got = _check(small, 1, 1, None)
+    gu.assert_within("o", tree_attn(q, c).cpu(), gu.step(q, small, None, 32 ** -0.5))
+
+
 @pytest.mark.parametrize("n,Hq", [(5, 4), (40, 4), (70, 4)])
 @pytest.mark.parametrize("lens", [[0, 0, 200], [2000, 3, 90]], ids=["short", "split"])
 def test_tokens_that_see_nothing_get_zeros(lens, n, Hq):
