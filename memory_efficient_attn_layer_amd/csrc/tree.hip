@@ -483,7 +483,7 @@ template <class E, int N, bool COOP>
 __global__ __launch_bounds__(256) void tree_combine_kernel(TreeParams p) {
   constexpr int L = N / 4, GR = 256 / L;
   __shared__ __attribute__((aligned(16))) float num_s[COOP ? GR : 1][COOP ? N : 4];
-  __shared__ float den_s[GR];
+  __shared__ float den_s[GR], max_s[GR];
   const int G = p.Hq / p.c.Hkv, R = p.n * G, tid = threadIdx.x, gi = tid / L, d = tid % L * 4;
   const int s = blockIdx.x, row = COOP ? blockIdx.y : blockIdx.y * GR + gi;  // row: kv * R + r
   const int* head = reinterpret_cast<const int*>(p.part) + 2 * s;
@@ -491,31 +491,60 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeParams p) {
   if (count <= 1 || row >= p.c.Hkv * R) return;  // written by the first launch (COOP: uniform)
   const size_t pitch = (size_t)p.c.Hkv * R * (N + 4);
   const float* part = p.part + tree_head_floats(p.c.seqs) + ((size_t)item * p.c.Hkv * R + row) * (N + 4);
-  float M = -INFINITY;
-  for (int i = tid % L; i < count; i += L) M = fmaxf(M, part[i * pitch + N]);
-#pragma unroll
-  for (int off = 1; off < L; off <<= 1) M = fmaxf(M, shfl_xor(M, off));
+  // Eight chunks at a time, all their loads in flight together; what was added so far
+  // is scaled down where they have a larger maximum. (33 chunks of one token, the whole
+  // call: 13.7 us; 15.3 with the maximum looked up first.)
+  float M = -INFINITY, den = 0.f;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
-  float den = 0.f;
-#pragma unroll 8
-  for (int i = COOP ? gi : 0; i < count; i += COOP ? GR : 1) {
-    const float* ps = part + i * pitch;
-    const f32x4 ml = *reinterpret_cast<const f32x4*>(ps + N), x = *reinterpret_cast<const f32x4*>(ps + d);
-    // (A chunk without weights holds zeros: its weight is made 0, not exp2(-inf + inf).)
-    const float w = ml[1] == 0.f ? 0.f : ml[0] == M ? 1.f : exp2f(ml[0] - M);
-    den = __builtin_fmaf(w, ml[1], den);
+  constexpr int STEP = COOP ? GR : 1;
+  for (int i0 = COOP ? gi : 0; i0 < count; i0 += 8 * STEP) {
+    f32x4 ml[8], x[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) num[e] = __builtin_fmaf(w, x[e], num[e]);
+    for (int u = 0; u < 8; ++u) {
+      const float* ps = part + (i0 + u * STEP) * pitch;
+      ml[u] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+      x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (i0 + u * STEP < count) {
+        ml[u] = *reinterpret_cast<const f32x4*>(ps + N);
+        x[u] = *reinterpret_cast<const f32x4*>(ps + d);
+      }
+    }
+    float mx = M;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) mx = fmaxf(mx, ml[u][0]);
+    const float a = M == mx ? 1.f : exp2f(M - mx);
+    num *= a;
+    den *= a;
+    M = mx;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      // (A chunk without weights holds zeros: its weight is made 0, not exp2(-inf + inf).)
+      if (ml[u][1] == 0.f) continue;
+      const float w = ml[u][0] == M ? 1.f : exp2f(ml[u][0] - M);
+      den = __builtin_fmaf(w, ml[u][1], den);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) num[e] = __builtin_fmaf(w, x[u][e], num[e]);
+    }
   }
   if (COOP) {
     *reinterpret_cast<f32x4*>(&num_s[gi][d]) = num;
-    if (d == 0) den_s[gi] = den;
+    if (d == 0) {
+      den_s[gi] = den;
+      max_s[gi] = M;
+    }
     __syncthreads();
     if (gi != 0) return;
+    float mx = M;
+#pragma unroll
+    for (int g = 1; g < GR; ++g) mx = fmaxf(mx, max_s[g]);
+    const float a = M == mx ? 1.f : exp2f(M - mx);
+    num *= a;
+    den *= a;
 #pragma unroll
     for (int g = 1; g < GR; ++g) {
-      num += *reinterpret_cast<const f32x4*>(&num_s[g][d]);
-      den += den_s[g];
+      const float b = max_s[g] == mx ? 1.f : exp2f(max_s[g] - mx);
+      num += b * *reinterpret_cast<const f32x4*>(&num_s[g][d]);
+      den = __builtin_fmaf(b, den_s[g], den);
     }
   }
   const float inv = den == 0.f ? 0.f : 1.0f / den;
