@@ -334,6 +334,7 @@ int mea_tree_attn(const mea_paged* c, int64_t n, int64_t Hq, float scale, const 
   p.Hq = (int)Hq;
   const mea::TreeGrid g = tree_grid_of(c, n, Hq);
   p.want = g.want;
+  p.least = g.least;
   p.full = g.full;
   p.row_groups = g.row_groups;
   p.sl2e = scale * 1.4426950408889634f;

@@ -87,7 +87,7 @@ struct TreeParams {
   int64_t q_seq, q_tok, q_head;
   const unsigned char* mask;  // (n, n) bytes per sequence, mask_seq apart (0: one for all); null: causal
   int64_t mask_seq;
-  int n, Hq, want, full, row_groups;  // the last three: of TreeGrid
+  int n, Hq, want, least, full, row_groups;  // from want on: of TreeGrid
   float sl2e;
   bits16* o;    // (seqs, n, Hq, N)
   // Null where no sequence can have two chunks: first item and chunks of each
@@ -99,7 +99,7 @@ __host__ __device__ inline size_t tree_head_floats(int seqs) { return (2 * (size
 // can have; split: a sequence may have several chunks, whose sums the second launch
 // joins.
 struct TreeGrid {
-  int blocks, row_groups, turn, want, full;
+  int blocks, row_groups, turn, want, least, full;
   int64_t items;
   bool split;
 };

@@ -86,8 +86,8 @@ constexpr int kManySeqs = 4096;
 struct Chunk {
   int size, seq, chunk, count;  // seq < 0: no such item; count: the sequence's chunks (0 where it has no row)
 };
-// want, full: of TreeGrid; turn: granule of the size.
-__device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int turn, int full, int item) {
+// want, least, full: of TreeGrid; turn: granule of the size.
+__device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int turn, int least, int full, int item) {
   const int lane = threadIdx.x & 63;
   auto len = [&](int s) { return min(max(c.lengths[s], 0), c.max_pages << c.lg_page); };
   Chunk r;
@@ -109,13 +109,10 @@ __device__ __forceinline__ Chunk find_chunk(const PagedCache& c, int want, int t
   auto whole = [&](int keys) { return (keys + turn - 1) / turn * turn; };
   auto chunks = [&](int n) { return max((n + r.size - 1) / r.size, 1); };
   // Few sequences: as many chunks as run at one time. Many: four times as many, which
-  // even out the rounds, but none below kLeast keys, which a workgroup's start and the
-  // sums' way through memory would cost more than (64 sequences of up to 1024 rows of
-  // 8 heads, one token: chunks of 150 keys 61 us, whole sequences 48; of up to 2048:
-  // 90 and 82). (Sums of keys in units of 16, so that they fit 32 bits.)
+  // even out the rounds. (Sums of keys in units of 16, so that they fit 32 bits.)
   const bool few = 2 * c.seqs <= want;
   const int total = wave_add(sum([](int n) { return (n + 15) >> 4; })), parts = few ? want : 4 * want;
-  r.size = min(max(whole(((total + parts - 1) / parts) << 4), few ? 2 * turn : kLeast), kMaxChunk);
+  r.size = min(max(whole(((total + parts - 1) / parts) << 4), least), kMaxChunk);
   while (few && r.size < kMaxChunk && wave_add(sum(chunks)) > want) r.size = min(whole(r.size + r.size / 16), kMaxChunk);
   // Item -> (sequence, chunk): every sequence has one item at least.
   const int own = sum(chunks), up = wave_scan(own);
@@ -156,7 +153,7 @@ __global__ __launch_bounds__((64 * Tile<N, RW>::WAVES), RW == 1 || N == 256 ? 1 
   const int G = p.Hq / cc.Hkv, R = p.n * G;
   // Key heads fastest, then the row groups that read the same rows, then chunks.
   const int kv = blockIdx.x % cc.Hkv, grp = blockIdx.x / cc.Hkv, item = grp / p.row_groups;
-  const Chunk ck = find_chunk(cc, p.want, T::TURN, p.full, item);
+  const Chunk ck = find_chunk(cc, p.want, T::TURN, p.least, p.full, item);
   if (ck.seq < 0) return;
   const int s = ck.seq;
   const int len = __builtin_amdgcn_readfirstlane(min(max(cc.lengths[s], 0), cc.max_pages << cc.lg_page));
@@ -618,6 +615,7 @@ TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
   const int64_t full = (int64_t)seqs * g.full;
   if (seqs > kManySeqs || (int64_t)seqs * (capacity / 16 + 1) >= INT64_C(1) << 31) {
     g.want = 0;
+    g.least = kMaxChunk;
     g.items = full;
     g.split = capacity > kMaxChunk;
     return g;
@@ -625,13 +623,18 @@ TreeGrid tree_grid(int seqs, int Hkv, int rows, int capacity, int N) {
   // Few sequences: at most `want` chunks, many: 4 * want and one for each; or the
   // largest chunks, if they are more; no more than the capacity has of the smallest.
   g.want = (int)(slots / lanes > 1 ? slots / lanes : 1);
+  // Keys of a chunk at least. Many sequences: what a workgroup's start and the sums' way
+  // through memory are worth (64 sequences of up to 1024 rows of 8 heads, one token:
+  // chunks of 150 keys 61 us, whole sequences 48; of up to 2048: 90 and 82). Few: two
+  // turns, or one where its sums are small beside its keys (N = 128, one sequence of
+  // 4096 rows, 4 query rows a head: 13.6 us with two, 13.1 with one; 64: 16.4 and 19.0).
   const bool few = 2 * seqs <= g.want;
-  const int least = few ? 2 * g.turn : kLeast;
-  const int64_t most = (int64_t)seqs * ((capacity + least - 1) / least);
+  g.least = !few ? kLeast : 4 * rows <= g.turn ? g.turn : 2 * g.turn;
+  const int64_t most = (int64_t)seqs * ((capacity + g.least - 1) / g.least);
   g.items = few ? g.want : 4 * g.want + seqs;
   if (g.items < full) g.items = full;
   if (g.items > most) g.items = most;
-  g.split = capacity > least;
+  g.split = capacity > g.least;
   return g;
 }
 
