@@ -102,4 +102,16 @@ __device__ __forceinline__ void add_not_finite(f32x16& o, const bf16_bits* row, 
   }
 }
 
+// Inclusive sum over the wave's lanes, every lane taking part: within rows of sixteen
+// lanes by DPP row shifts, then the last lane of a row, and of half a wave, to those behind.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
 }  // namespace mea

@@ -63,17 +63,6 @@ __device__ __forceinline__ void wait_loads() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// Inclusive sum over the wave's lanes, every lane taking part: within rows of sixteen
-// lanes by DPP row shifts, then the last lane of a row, and of half a wave, to those behind.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-  return v;
-}
 // (By a permute, not a scalar register: the loop's counts in scalars cost the kernel spills.)
 __device__ __forceinline__ int wave_add(int v) { return __shfl(wave_scan(v), 63, 64); }
 
