@@ -503,7 +503,7 @@ __global__ __launch_bounds__(256, N <= 64 ? 3 : N == 256 ? 1 : 2) void grouped_d
     // On the diagonal, where a sequence's first rows have all their keys, what rounding ds
     // left goes in as well: few keys leave few errors to even out (sequences of 1 to 5
     // tokens: dq and dk 2.5e-3 off their norms without it, 1.9e-3 with it, 1.7e-3 if
-    // nothing but the outputs were rounded; 1% of the backward's time at 1100 tokens).
+    // nothing but the outputs were rounded; 1% of forward and backward at 1100 tokens).
     u32x4 rest[2];
     if (MASK) {
 #pragma unroll
